@@ -115,6 +115,14 @@ struct GemmArgs {
   uint32_t ln_nt = 0;
   const float* ln_s = nullptr;
   float ln_eps = 0.0f;
+  // Optional low-rank adapters (dense A, B_NK): the accumulator of row m also
+  // takes sum_r lo_t[m][r] lo_up[a][n][r], a = lo_ids[m / lo_run], where a is
+  // in [0, lo_n).  lo_t: [M][lo_ld] of elem, columns lo_rank to lo_ld - 1 zero
+  // (lo_ld: lo_rank rounded up to a 16-byte vector); lo_up: [lo_n][N][lo_rank].
+  const void* lo_t = nullptr;
+  const void* lo_up = nullptr;
+  const int32_t* lo_ids = nullptr;
+  uint32_t lo_n = 0, lo_rank = 0, lo_ld = 0, lo_run = 1;
   // Set by launch_gemm: fp16 NHWC output whose rows, bias, temb bias and
   // residual allow 16-byte vectors (the C tile is then staged through LDS
   // and written 8 columns per thread).
@@ -212,6 +220,12 @@ uint32_t gemm_rstats_tiles(const GemmArgs& g, int tile_cfg);
 // Whether launch_gemm applies the LayerNorm fold of g.ln_* (fp16 vector
 // epilogue, batch 1, no GroupNorm statistics; split-K included).
 bool gemm_lnfold_ok(const GemmArgs& g, int elem, int tile_cfg);
+// lo_t of the adapters (k_lora.hip): t[m][r] = scale[a] sum_k x[m][k] down[a][r][k]
+// in elem, a = ids[m / run], for the rows whose a is in [0, n); others are left.
+// scale may be null (ones).
+void launch_lora_down(const void* x, const void* down, const float* scale, const int32_t* ids, void* t,
+                      uint32_t M, uint32_t K, uint32_t n, uint32_t rank, uint32_t ld, uint32_t run,
+                      int elem, int num_cus, hipStream_t s);
 // OIHW (any dtype) -> OHWI fp16 with optional zero channel padding Cin -> Cin_pad.
 void launch_repack_oihw_ohwi(hipStream_t s, const void* w, int wdt, void* out, uint32_t Cout,
                              uint32_t Cin, uint32_t ks, uint32_t Cin_pad);

@@ -1,0 +1,619 @@
+// Flash attention to an encoder's states: any head size up to 256, lengths per
+// batch entry, additive biases, query heads that share key heads; fp16 on the
+// fp16 MFMA, fp32 on the fp32 MFMA.
+//
+//   o = softmax(scale q k^T + bias) v
+//
+// Rows.  The G query heads that share a key head are rows beside its queries:
+// row = query * G + head, so that one read of a key serves all of them, and a
+// single token's heads fill a 16-row MFMA tile together.
+//
+// MFMA mapping, as in k_attn.hip: S^T = K Q'^T with Q' = q * scale * log2(e)
+// (in the tensors' type), so scores come out in log2 units with the C layout
+// leaving lane l row l%16 and keys 4g..4g+3 (g = l/16) of each 16-key tile;
+// O^T += V^T P^T takes those probabilities as its B operand without moving
+// them.  fp16: v_mfma_f32_16x16x32_f16, the V^T operand by transposed LDS
+// reads.  fp32: v_mfma_f32_16x16x4_f32 on four registers of a 16-byte read,
+// whose k index runs over channels (keys) 4g + j for j = 0..3.
+//
+// Softmax in one pass: a running maximum m per row, taken from the first keys
+// that a row has and raised only when a lane's probabilities of a tile pass
+// 2^15 (fp16-safe), then the tile is redone; row sums once, at the end.  m stays
+// at kNone until a row has seen a key, so rows that a mask leaves empty end
+// with a zero sum and store zeros.
+//
+// Keys come in tiles of KT through LDS (loads go straight to LDS; 16-byte
+// chunks XOR-swizzled by row so that fragment reads meet no bank twice), two
+// buffers, the next tile in flight while one is computed.  Rows are padded to
+// DK channels in registers and to a power of two of chunks in LDS; chunks past
+// d and keys past the length are never read from memory and land as zeros.
+//
+// WM wavefronts share a tile, each with QG groups of 16 rows; WK such groups
+// of wavefronts walk different tiles of the same rows and are merged through
+// LDS.  Many rows: WM = 4, WK = 1.  Few rows (a token, a handful of
+// latents): WM = 1, WK = 4, so that every wavefront streams keys of its own.
+// Where the rows still leave CUs idle the keys are split over workgroups as
+// well and k_attn_enc_merge joins the parts.
+#pragma once
+
+#include <type_traits>
+
+#include "di_attn_enc.h"
+#include "di_device.h"
+
+namespace di {
+
+namespace {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr float kNone = -3.402823466e38f;  // maximum of a row without a key so far
+constexpr float kSwamped = -1e30f;         // a bias that replaces its score
+constexpr float kLowest = -3.0e38f;        // the lowest one in log2 units: above kNone
+// a lane's probabilities of one tile sum to at most this without a rescale,
+// so none exceeds it either (fp16 max is 65504)
+constexpr uint32_t kLaneSumMaxBits = 0x47000000u;  // 32768.0f
+constexpr float kLog2E = 1.4426950408889634f;
+constexpr int kWaitAll = (7 << 4);  // s_waitcnt vmcnt(0) lgkmcnt(0), expcnt not waited on
+
+template <int N>
+using Int = std::integral_constant<int, N>;
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t enc_rsrc(const void* p, uint32_t bytes) {
+  // raw buffer, stride 0; dword3 0x00020000 is the gfx9-family data format
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)bytes, 0x00020000);
+}
+
+// 16 bytes per lane at off of r straight to LDS, lane l's at p + 16 l
+__device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, unsigned char* p, uint32_t off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)p, 16, off, 0, 0, 0);
+}
+
+// lanes l, l^16, l^32, l^48 hold the same row
+__device__ __forceinline__ float enc_max4(float x) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float enc_sum4(float x) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Shapes of one instantiation.
+template <typename T, int DK, bool FEW>
+struct EncShape {
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int EPC = 16 / sizeof(T);  // elements per 16-byte chunk
+  // chunks of an LDS row: a power of two
+  static constexpr int C0 = DK / EPC;
+  static constexpr int CPR = C0 <= 4 ? 4 : C0 <= 8 ? 8 : C0 <= 16 ? 16 : C0 <= 32 ? 32 : 64;
+  // keys per tile: K and V tile of at most 32 KiB together (16 KiB for few rows)
+  static constexpr int KT = FEW ? (CPR <= 16 ? 32 : F32 ? 16 : 32)
+                                : (CPR <= 16 ? 64 : CPR == 32 ? 32 : 16);
+  static constexpr int TILE = KT * CPR * 16;  // bytes of a K (V) tile
+  static constexpr int WM = FEW ? 1 : 4;
+  // four wavefronts' buffers while they fit the 160 KiB of LDS
+  static constexpr int WK = FEW ? (TILE * 4 * 4 <= 128 * 1024 ? 4 : 2) : 1;
+  static constexpr int QG = FEW || F32 || DK > 128 ? 1 : 2;
+  static constexpr int ROWS = WM * QG * 16;
+  static constexpr int NT = WM * WK * 64;
+  static constexpr int LDS = WK * 4 * TILE;  // [key group][buffer][K | V]
+  // wavefronts per SIMD that registers are kept for: what the LDS lets reside
+  static constexpr int WAVES = LDS * 2 <= 160 * 1024 ? 2 : 1;
+};
+
+template <typename T, int DK, bool FEW, bool BIAS>
+__global__ __launch_bounds__((EncShape<T, DK, FEW>::NT), (EncShape<T, DK, FEW>::WAVES))
+void k_attn_enc(AttnEncArgs a) {
+  typedef EncShape<T, DK, FEW> Sh;
+  constexpr bool F32 = Sh::F32;
+  constexpr int EPC = Sh::EPC, CPR = Sh::CPR, KT = Sh::KT, TILE = Sh::TILE, WM = Sh::WM, WK = Sh::WK;
+  constexpr int QG = Sh::QG, NKT = KT / 16, NDT = DK / 16;
+  constexpr int RB = CPR * 16;                // bytes of an LDS row
+  constexpr int QC = F32 ? DK / 16 : DK / 32; // K fragment reads per 16-key tile
+  __shared__ __attribute__((aligned(16))) unsigned char smem[Sh::LDS];
+  kernarg_warm(a);
+
+  const uint32_t tid = threadIdx.x, lane = tid & 63;
+  const uint32_t wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t wm = wv % WM, kg = wv / WM;
+  const uint32_t r = lane & 15, g = lane >> 4;
+
+  // XCD-aware numbering: block i runs on XCD i % 8; XCD x takes the x-th
+  // contiguous run of the work list, so a head's keys stay in one L2
+  const uint32_t T_ = gridDim.x, bid = blockIdx.x, xcd = bid & 7u, idx = bid >> 3;
+  const uint32_t per = T_ >> 3, extra = T_ & 7u;
+  const uint32_t w = xcd < extra ? xcd * (per + 1) + idx : extra * (per + 1) + (xcd - extra) * per + idx;
+  const uint32_t mb = w % a.blocks, rest = w / a.blocks, split = rest % a.splits, hb = rest / a.splits;
+  const uint32_t h = hb % a.Hk, b = hb / a.Hk;
+
+  // this entry's keys; its tiles [t0, t1) of this workgroup's range and key group
+  uint32_t nk = a.Skv;
+  if (a.len) {
+    const int n = a.len[b];
+    nk = n <= 0 ? 0u : min((uint32_t)n, a.Skv);
+  }
+  nk = __builtin_amdgcn_readfirstlane(nk);
+  const int n_tiles = (int)((nk + KT - 1) / KT);
+  const int tps = (n_tiles + (int)a.splits - 1) / (int)a.splits;
+  const int w0 = min((int)split * tps, n_tiles), w1 = min(w0 + tps, n_tiles);
+  const int tpg = (w1 - w0 + WK - 1) / WK;
+  const int t0 = min(w0 + (int)kg * tpg, w1), t1 = min(t0 + tpg, w1);
+
+  const T* K = (const T*)a.k + b * a.bk + h * a.hk;
+  const T* V = (const T*)a.v + b * a.bv + h * a.hv;
+
+  // rows of this lane
+  uint32_t row[QG], qh[QG], qi_[QG];
+  bool live[QG];
+#pragma unroll
+  for (int i = 0; i < QG; i++) {
+    row[i] = mb * Sh::ROWS + (wm * QG + i) * 16 + r;
+    live[i] = row[i] < a.rows;
+    const uint32_t rr = live[i] ? row[i] : 0;
+    qi_[i] = a.G == 1 ? rr : rr / a.G;
+    qh[i] = h * a.G + (rr - qi_[i] * a.G);
+  }
+
+  // Q' fragments: fp16 lane (r, g) channels 32 c + 8 g .. + 7, fp32 16 c + 4 g .. + 3
+  typedef typename std::conditional<F32, f32x4, f16x8>::type frag;
+  frag qf[QG][QC];
+#pragma unroll
+  for (int i = 0; i < QG; i++) {
+    const T* p = (const T*)a.q + b * a.bq + qh[i] * a.hq + (uint64_t)qi_[i] * a.ldq;
+#pragma unroll
+    for (int c = 0; c < QC; c++) {
+      const uint32_t e = (c * 4 + g) * EPC;
+      frag t = {};
+      if (live[i] && e < a.d) t = *(const frag*)(p + e);
+#pragma unroll
+      for (int j = 0; j < EPC; j++) qf[i][c][j] = (T)((float)t[j] * a.scale_log2);
+    }
+  }
+  const float* bp[QG];
+  if constexpr (BIAS) {
+#pragma unroll
+    for (int i = 0; i < QG; i++)
+      bp[i] = a.bias + b * a.bias_b + qh[i] * a.bias_h + qi_[i] * a.bias_q;
+  }
+
+  // LDS swizzles, on 16-byte chunks.  K: the 16 rows that one pass of a
+  // fragment read takes at one chunk land on all 64 banks.  V, fp16: a
+  // 32-lane pass of a transposed read covers 8 rows x 2 chunks; fp32: the four
+  // rows 4g + j of a read cover 64 bytes each.
+  auto kswz = [](uint32_t row) -> uint32_t {
+    if constexpr (CPR == 4) return (row >> 2) & 3u;
+    else if constexpr (CPR == 8) return (row >> 1) & 7u;
+    else return row & 15u;
+  };
+  auto vswz = [](uint32_t row) -> uint32_t {
+    if constexpr (F32) return (((row >> 2) & 3u) << 2) & (CPR - 1);
+    else if constexpr (CPR == 4) return ((row >> 2) & 1u) << 1;
+    else if constexpr (CPR == 8) return row & 7u;
+    else return (row & 7u) << 1;
+  };
+
+  // loads of a tile: 64 chunks (1 KiB of LDS) per instruction, lane l's chunk
+  // at base + 16 l; a chunk past d gets an offset out of range
+  constexpr int NI = TILE / (1024 * WM);
+  static_assert(NI >= 1 && NI * 1024 * WM == TILE, "whole instructions per wavefront");
+  uint32_t dk[NI], dv[NI];
+#pragma unroll
+  for (int i = 0; i < NI; i++) {
+    const uint32_t f = (wm * NI + i) * 64 + lane, kr = f / CPR, sl = f % CPR;
+    const uint32_t ck = sl ^ kswz(kr), cv = sl ^ vswz(kr);
+    dk[i] = ck * EPC < a.d ? kr * (uint32_t)(a.ldk * sizeof(T)) + ck * 16u : 0x80000000u;
+    dv[i] = cv * EPC < a.d ? kr * (uint32_t)(a.ldv * sizeof(T)) + cv * 16u : 0x80000000u;
+  }
+  auto fetch = [&](int t, auto buf_c) {
+    const uint32_t key0 = (uint32_t)t * KT, left = min(nk - key0, (uint32_t)KT);
+    const __amdgpu_buffer_rsrc_t rK = enc_rsrc(K + (uint64_t)key0 * a.ldk,
+                                               (uint32_t)(((left - 1) * a.ldk + a.d) * sizeof(T)));
+    const __amdgpu_buffer_rsrc_t rV = enc_rsrc(V + (uint64_t)key0 * a.ldv,
+                                               (uint32_t)(((left - 1) * a.ldv + a.d) * sizeof(T)));
+    unsigned char* base = smem + (kg * 2 + decltype(buf_c)::value) * 2 * TILE + wm * NI * 1024;
+#pragma unroll
+    for (int i = 0; i < NI; i++)
+      load_lds16(rK, base + i * 1024, dk[i]);
+#pragma unroll
+    for (int i = 0; i < NI; i++)
+      load_lds16(rV, base + TILE + i * 1024, dv[i]);
+  };
+
+  // K fragment c of 16-key tile kt: row kt * 16 + r, chunk 4 c + g
+  uint32_t k_rd[QC];
+#pragma unroll
+  for (int c = 0; c < QC; c++) k_rd[c] = r * RB + (((4 * c + g) ^ kswz(r)) << 4);
+  // V^T fragments.  fp16, 16 channels dt: lane r of group g reads 4 channels
+  // of row 4g + r/4 at 16 dt + 4 (r%4).  fp32: channel 16 dt + r of row 4g + j.
+  uint32_t v_rd[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; dt++) {
+    if constexpr (F32)
+      v_rd[dt] = TILE + 4 * g * RB + (((4 * dt + (r >> 2)) ^ vswz(4 * g)) << 4) + (r & 3) * 4;
+    else
+      v_rd[dt] = TILE + (4 * g + (r >> 2)) * RB +
+                 (((2 * dt + ((r & 3) >> 1)) ^ vswz(4 * g + (r >> 2))) << 4) + (r & 1) * 8;
+  }
+
+  float m[QG], l[QG];
+  f32x4 o[QG][NDT];
+#pragma unroll
+  for (int i = 0; i < QG; i++) {
+    m[i] = kNone;
+    l[i] = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < NDT; dt++) o[i][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  auto tile = [&](auto cur_c, int t) {
+    constexpr int cur = decltype(cur_c)::value;
+    const unsigned char* sb = smem + (kg * 2 + cur) * 2 * TILE;
+    if (t < t1) {
+      if (t + 1 < t1) fetch(t + 1, Int<cur ^ 1>{});
+      const uint32_t key0 = (uint32_t)t * KT;
+      const bool ragged = key0 + KT > nk;
+      f32x4 bb[BIAS ? QG : 1][BIAS ? NKT : 1];
+      if constexpr (BIAS) {
+        // in flight while the scores are computed; past the last key: unread
+#pragma unroll
+        for (int i = 0; i < QG; i++)
+#pragma unroll
+          for (int kt = 0; kt < NKT; kt++) {
+            const uint32_t key = key0 + kt * 16 + 4 * g;
+            if (!ragged) {
+              bb[i][kt] = *(const f32x4u*)(bp[i] + key);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; j++) bb[i][kt][j] = key + j < nk ? bp[i][key + j] : -INFINITY;
+            }
+          }
+      }
+      f32x4 s[QG][NKT];
+#pragma unroll
+      for (int kt = 0; kt < NKT; kt++) {
+#pragma unroll
+        for (int i = 0; i < QG; i++) s[i][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < QC; c++) {
+          const frag kf = *(const frag*)(sb + k_rd[c] + kt * 16 * RB);
+#pragma unroll
+          for (int i = 0; i < QG; i++) {
+            if constexpr (F32) {
+#pragma unroll
+              for (int j = 0; j < 4; j++)
+                s[i][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qf[i][c][j], s[i][kt], 0, 0, 0);
+            } else {
+              s[i][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[i][c], s[i][kt], 0, 0, 0);
+            }
+          }
+        }
+      }
+      if (ragged) {
+#pragma unroll
+        for (int kt = 0; kt < NKT; kt++)
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            if (key0 + kt * 16 + 4 * g + j >= nk) {
+#pragma unroll
+              for (int i = 0; i < QG; i++) s[i][kt][j] = -INFINITY;
+            }
+      }
+      bool removed = false;  // some query of this wavefront does not see some key
+      if constexpr (BIAS) {
+#pragma unroll
+        for (int i = 0; i < QG; i++)
+#pragma unroll
+          for (int kt = 0; kt < NKT; kt++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const float x = bb[i][kt][j];
+              removed |= x == -INFINITY;
+              if (x <= kSwamped) s[i][kt][j] = 0.0f;  // whatever the score: it may be NaN
+              // in log2 units; the product of a finite bias stays finite
+              bb[i][kt][j] = x == -INFINITY ? x : fmaxf(x * kLog2E, kLowest);
+            }
+      }
+      auto score = [&](int i, int kt, int j) -> float {
+        if constexpr (BIAS) return s[i][kt][j] + bb[i][kt][j];
+        else return s[i][kt][j];
+      };
+      // raise the running maximum to this tile's where that is larger
+      auto raise = [&](int i) {
+        float mx = score(i, 0, 0);
+#pragma unroll
+        for (int kt = 0; kt < NKT; kt++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) mx = fmaxf(mx, score(i, kt, j));
+        mx = fmaxf(enc_max4(mx), m[i]);
+        const float al = m[i] == kNone ? 0.0f : __builtin_amdgcn_exp2f(m[i] - mx);
+        m[i] = mx;
+        l[i] *= al;
+#pragma unroll
+        for (int dt = 0; dt < NDT; dt++) o[i][dt] *= al;
+      };
+      float pr[QG][NKT][4], ts[QG];
+      auto probs = [&](int i) {
+        ts[i] = 0.0f;
+#pragma unroll
+        for (int kt = 0; kt < NKT; kt++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            // with a bias, (bias - m) first: it is exact where they are close
+            const float x = BIAS ? s[i][kt][j] + (bb[i][kt][j] - m[i]) : s[i][kt][j] - m[i];
+            pr[i][kt][j] = __builtin_amdgcn_exp2f(x);
+            ts[i] += pr[i][kt][j];
+          }
+      };
+#pragma unroll
+      for (int i = 0; i < QG; i++) {
+        // rows without a key so far: take the maximum
+        if (__builtin_amdgcn_ballot_w64(m[i] == kNone) != 0) raise(i);
+        probs(i);
+        // a probability above 2^15 (or inf / NaN) shows in its lane's sum; the
+        // bits' order puts finite < inf < NaN
+        if (__builtin_amdgcn_ballot_w64((__float_as_uint(ts[i]) & 0x7fffffffu) > kLaneSumMaxBits) != 0) {
+          raise(i);
+          probs(i);
+        }
+        l[i] += ts[i];
+      }
+      // O^T += V^T P^T.  MASKED: the values of keys that none of this
+      // wavefront's rows sees become zeros (0 * NaN would not vanish).
+      uint32_t seen = ~0u;  // bit 4 kt + j: key kt * 16 + 4g + j
+      if constexpr (BIAS) {
+        if (__builtin_amdgcn_ballot_w64(removed) != 0) {
+          seen = 0;
+#pragma unroll
+          for (int kt = 0; kt < NKT; kt++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              bool some = false;
+#pragma unroll
+              for (int i = 0; i < QG; i++) some |= live[i] && bb[i][kt][j] > -INFINITY;
+              const uint64_t bal = __builtin_amdgcn_ballot_w64(some);
+              seen |= (((bal >> (16 * g)) & 0xffffu) != 0 ? 1u : 0u) << (4 * kt + j);
+            }
+        }
+      }
+      auto pv = [&](auto masked_c) {
+        constexpr bool MASKED = decltype(masked_c)::value != 0;
+        if constexpr (F32) {
+#pragma unroll
+          for (int kt = 0; kt < NKT; kt++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+              for (int dt = 0; dt < NDT; dt++) {
+                float vf = *(const float*)(sb + v_rd[dt] + (kt * 16 + j) * RB);
+                if constexpr (MASKED) vf = (seen >> (4 * kt + j)) & 1u ? vf : 0.0f;
+#pragma unroll
+                for (int i = 0; i < QG; i++)
+                  o[i][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf, pr[i][kt][j], o[i][dt], 0, 0, 0);
+              }
+        } else {
+#pragma unroll
+          for (int c = 0; c < NKT / 2; c++) {
+            f16x8 pf[QG];
+#pragma unroll
+            for (int i = 0; i < QG; i++)
+#pragma unroll
+              for (int j = 0; j < 8; j++) pf[i][j] = (f16)pr[i][2 * c + j / 4][j % 4];
+            u32x4 keep = {~0u, ~0u, ~0u, ~0u};
+            if constexpr (MASKED) {
+#pragma unroll
+              for (int j = 0; j < 4; j++)
+                keep[j] = ((seen >> (8 * c + 2 * j)) & 1u ? 0xffffu : 0u) |
+                          ((seen >> (8 * c + 2 * j + 1)) & 1u ? 0xffff0000u : 0u);
+            }
+#pragma unroll
+            for (int dt = 0; dt < NDT; dt++) {
+              const unsigned char* vp = sb + v_rd[dt] + c * 32 * RB;
+              const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)vp);
+              const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vp + 16 * RB));
+              f16x8 vf = __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+              if constexpr (MASKED)
+                vf = __builtin_bit_cast(f16x8, __builtin_bit_cast(u32x4, vf) & keep);
+#pragma unroll
+              for (int i = 0; i < QG; i++)
+                o[i][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[i], o[i][dt], 0, 0, 0);
+            }
+          }
+        }
+      };
+      if (BIAS && __builtin_amdgcn_ballot_w64(removed) != 0) pv(Int<1>{});
+      else pv(Int<0>{});
+    }
+    // the next tile has landed, and every wavefront that shares it is done with
+    // this one (a wavefront with tiles of its own waits for itself alone)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_waitcnt(kWaitAll);
+    if constexpr (WM > 1) __builtin_amdgcn_s_barrier();
+    else __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  };
+
+  if (t0 < t1) fetch(t0, Int<0>{});
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __builtin_amdgcn_s_waitcnt(kWaitAll);
+  __syncthreads();
+  // two tiles per iteration so that each LDS buffer has fixed offsets; every
+  // wavefront of the workgroup makes tpg iterations
+  for (int i = 0; i < tpg; i += 2) {
+    tile(Int<0>{}, t0 + i);
+    if (i + 1 < tpg) tile(Int<1>{}, t0 + i + 1);
+  }
+#pragma unroll
+  for (int i = 0; i < QG; i++) l[i] = enc_sum4(l[i]);
+
+  if constexpr (WK > 1) {
+    // merge the key groups: groups 1.. leave (o, m, l) in LDS, float f of lane
+    // l at [f][l]; group 0 rescales every part to the largest maximum
+    static_assert(WK == 1 || QG == 1, "key groups with one row group");
+    constexpr int NF = NDT * 4 + 2;
+    static_assert((WK - 1) * WM * NF * 64 * 4 <= (int)sizeof(smem), "the parts fit the buffers");
+    float* xs = reinterpret_cast<float*>(smem);
+    __syncthreads();  // the buffers are free
+    if (kg > 0) {
+      float* dst = xs + ((kg - 1) * WM + wm) * NF * 64 + lane;
+#pragma unroll
+      for (int dt = 0; dt < NDT; dt++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) dst[(dt * 4 + j) * 64] = o[0][dt][j];
+      dst[NDT * 4 * 64] = m[0];
+      dst[(NDT * 4 + 1) * 64] = l[0];
+    }
+    __syncthreads();
+    if (kg > 0) return;
+    float mx = m[0];
+#pragma unroll
+    for (int k = 1; k < WK; k++) mx = fmaxf(mx, xs[((k - 1) * WM + wm) * NF * 64 + NDT * 4 * 64 + lane]);
+    float wk = __builtin_amdgcn_exp2f(m[0] - mx);
+    l[0] *= wk;
+#pragma unroll
+    for (int dt = 0; dt < NDT; dt++) o[0][dt] *= wk;
+#pragma unroll
+    for (int k = 1; k < WK; k++) {
+      const float* src = xs + ((k - 1) * WM + wm) * NF * 64 + lane;
+      wk = __builtin_amdgcn_exp2f(src[NDT * 4 * 64] - mx);
+      l[0] += src[(NDT * 4 + 1) * 64] * wk;
+#pragma unroll
+      for (int dt = 0; dt < NDT; dt++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[0][dt][j] += src[(dt * 4 + j) * 64] * wk;
+    }
+    m[0] = mx;
+  }
+
+  // lane (r, g) holds channels 16 dt + 4 g .. + 3 of its rows
+#pragma unroll
+  for (int i = 0; i < QG; i++) {
+    if (!live[i]) continue;
+    if (a.splits > 1) {
+      const uint64_t prow = (uint64_t)split * a.prows + (uint64_t)hb * a.rows + row[i];
+      float* dst = a.part_o + prow * a.d;
+#pragma unroll
+      for (int dt = 0; dt < NDT; dt++)
+        if (dt * 16 + g * 4 < a.d) *(f32x4*)(dst + dt * 16 + g * 4) = o[i][dt];
+      if (g == 0) *(float2*)(a.part_ml + prow * 2) = float2{m[i], l[i]};
+      continue;
+    }
+    const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
+    T* dst = (T*)a.o + b * a.bo + qh[i] * a.ho + (uint64_t)qi_[i] * a.ldo;
+#pragma unroll
+    for (int dt = 0; dt < NDT; dt++) {
+      if (dt * 16 + g * 4 >= a.d) continue;
+      const f32x4 v = o[i][dt] * inv;
+      if constexpr (F32) *(f32x4*)(dst + dt * 16 + g * 4) = v;
+      else *(f16x4*)(dst + dt * 16 + g * 4) = f16x4{(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3]};
+    }
+  }
+}
+
+// Joins the key ranges: one thread per 4 channels of a row, the ranges in order.
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_enc_merge(AttnEncArgs a) {
+  kernarg_warm(a);
+  const uint32_t vpr = a.d / 4;
+  const uint64_t total = a.prows * vpr, step = (uint64_t)gridDim.x * 256;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
+    const uint64_t row = i / vpr;
+    const uint32_t c = (uint32_t)(i - row * vpr) * 4;
+    float mx = kNone, l = 0.0f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t s0 = 0; s0 < a.splits; s0 += 4) {
+      float2 ml[4];
+      f32x4 v[4];
+#pragma unroll
+      for (uint32_t u = 0; u < 4; u++) {
+        const uint64_t p = (uint64_t)min(s0 + u, a.splits - 1) * a.prows + row;
+        ml[u] = *(const float2*)(a.part_ml + p * 2);
+        v[u] = *(const f32x4*)(a.part_o + p * a.d + c);
+      }
+      float m2 = mx;
+#pragma unroll
+      for (uint32_t u = 0; u < 4; u++) m2 = fmaxf(m2, ml[u].x);
+      const float al = __builtin_amdgcn_exp2f(mx - m2);
+      l *= al;
+      acc *= al;
+      mx = m2;
+#pragma unroll
+      for (uint32_t u = 0; u < 4; u++) {
+        if (s0 + u >= a.splits || ml[u].y == 0.0f) continue;  // (an empty range adds nothing)
+        const float wt = __builtin_amdgcn_exp2f(ml[u].x - mx);
+        l += wt * ml[u].y;
+        acc += wt * v[u];
+      }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const uint32_t rr = (uint32_t)(row % a.rows), q = rr / a.G;
+    const uint64_t hb = row / a.rows;
+    const uint64_t h = (hb % a.Hk) * a.G + (rr - q * a.G), b = hb / a.Hk;
+    T* dst = (T*)a.o + b * a.bo + h * a.ho + (uint64_t)q * a.ldo + c;
+    const f32x4 v = acc * inv;
+    if constexpr (sizeof(T) == 4) *(f32x4*)dst = v;
+    else *(f16x4*)dst = f16x4{(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3]};
+  }
+}
+
+template <typename T, int DK, bool FEW>
+void launch_enc_form(const AttnEncArgs& a, uint32_t B, hipStream_t s) {
+  const dim3 grid(a.blocks * a.splits * a.Hk * B);
+  if (a.bias) k_attn_enc<T, DK, FEW, true><<<grid, EncShape<T, DK, FEW>::NT, 0, s>>>(a);
+  else k_attn_enc<T, DK, FEW, false><<<grid, EncShape<T, DK, FEW>::NT, 0, s>>>(a);
+}
+
+template <typename T, int DK>
+void launch_enc_dk(const AttnEncArgs& a, uint32_t B, bool few, hipStream_t s) {
+  if (few) launch_enc_form<T, DK, true>(a, B, s);
+  else launch_enc_form<T, DK, false>(a, B, s);
+}
+
+// d padded to the channels of an instantiation
+inline uint32_t enc_channels(uint32_t d) { return d <= 192 ? (d + 31) / 32 * 32 : 256; }
+
+template <typename T, bool FEW>
+AttnEncForm enc_form(uint32_t d) {
+  auto of = [](auto s) {
+    typedef decltype(s) S;
+    return AttnEncForm{S::ROWS, S::KT, S::WK};
+  };
+  switch (enc_channels(d)) {
+    case 32: return of(EncShape<T, 32, FEW>{});
+    case 64: return of(EncShape<T, 64, FEW>{});
+    case 96: return of(EncShape<T, 96, FEW>{});
+    case 128: return of(EncShape<T, 128, FEW>{});
+    case 160: return of(EncShape<T, 160, FEW>{});
+    case 192: return of(EncShape<T, 192, FEW>{});
+    default: return of(EncShape<T, 256, FEW>{});
+  }
+}
+
+template <typename T>
+void launch_enc(const AttnEncArgs& a, uint32_t B, bool few, hipStream_t s) {
+  switch (enc_channels(a.d)) {
+    case 32: launch_enc_dk<T, 32>(a, B, few, s); break;
+    case 64: launch_enc_dk<T, 64>(a, B, few, s); break;
+    case 96: launch_enc_dk<T, 96>(a, B, few, s); break;
+    case 128: launch_enc_dk<T, 128>(a, B, few, s); break;
+    case 160: launch_enc_dk<T, 160>(a, B, few, s); break;
+    case 192: launch_enc_dk<T, 192>(a, B, few, s); break;
+    default: launch_enc_dk<T, 256>(a, B, few, s); break;
+  }
+  if (a.splits > 1) {
+    const uint64_t blocks = (a.prows * (a.d / 4) + 255) / 256;
+    k_attn_enc_merge<T><<<(uint32_t)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(a);
+  }
+}
+
+}  // namespace
+
+}  // namespace di

@@ -1,0 +1,110 @@
+// Attention to an encoder's states: the fp16 instantiations of k_attn_enc.h,
+// the choice of form and key split, and the C ABI (di_attn_encoder).
+#include <cmath>
+
+#include "di_views.h"
+#include "k_attn_enc.h"
+
+namespace di {
+
+void launch_attn_enc_f16(const AttnEncArgs& a, uint32_t B, bool few, hipStream_t s) {
+  launch_enc<f16>(a, B, few, s);
+}
+
+AttnEncForm attn_enc_form_f16(uint32_t d, bool few) {
+  return few ? enc_form<f16, true>(d) : enc_form<f16, false>(d);
+}
+
+}  // namespace di
+
+using namespace di;
+
+extern "C" int32_t di_attn_encoder(di_ctx* ctx, const di_heads* q, const di_heads* k, const di_heads* v,
+                                   const di_heads* o, di_handle kv_len, const di_attn_bias* bias,
+                                   uint32_t B, uint32_t Hq, uint32_t Hk, uint32_t Sq, uint32_t Skv,
+                                   uint32_t d, float scale, int32_t dt) {
+  const char* fn = "di_attn_encoder";
+  DI_REQUIRE(ctx != nullptr, DI_EINVAL, "null context");
+  DI_DTYPE(dt);
+  DI_REQUIRE(B && Hq && Hk && Sq && Skv && d, DI_EINVAL, "%s: zero dimension (B=%u Hq=%u Hk=%u Sq=%u Skv=%u d=%u)",
+             fn, B, Hq, Hk, Sq, Skv, d);
+  DI_REQUIRE(Hq % Hk == 0, DI_EINVAL, "%s: %u query heads over %u key heads", fn, Hq, Hk);
+  DI_REQUIRE(d % 8 == 0 && d <= 256, DI_EUNSUPPORTED, "%s: head dim %u (a multiple of 8 up to 256)", fn, d);
+  DI_REQUIRE(std::isfinite(scale), DI_EINVAL, "%s: scale %g", fn, (double)scale);
+  DI_REQUIRE(Skv < 1u << 31, DI_EUNSUPPORTED, "%s: %u keys", fn, Skv);
+  HeadsPtr pq, pk, pv, po;
+  int rc = check_heads(ctx, q, fn, "q", B, Sq, Hq, d, dt, &pq);
+  if (!rc) rc = check_heads(ctx, k, fn, "k", B, Skv, Hk, d, dt, &pk);
+  if (!rc) rc = check_heads(ctx, v, fn, "v", B, Skv, Hk, d, dt, &pv);
+  if (!rc) rc = check_heads(ctx, o, fn, "o", B, Sq, Hq, d, dt, &po);
+  if (rc) return rc;
+  DI_REQUIRE(heads_aligned(pq, 8) && heads_aligned(pk, 8) && heads_aligned(pv, 8) && heads_aligned(po, 8),
+             DI_EUNSUPPORTED, "%s: offsets and strides must be multiples of 8 elements", fn);
+  DI_REQUIRE(heads_distinct(po, B, Sq, Hq, d), DI_EINVAL, "%s: elements of o overlap", fn);
+  DI_REQUIRE(heads_apart(po, pq) && heads_apart(po, pk) && heads_apart(po, pv), DI_EINVAL, "%s: o overlaps an input",
+             fn);
+  // a tile's rows are addressed with 31-bit byte offsets from its first key
+  DI_REQUIRE(pk.token < 1ull << 22 && pv.token < 1ull << 22, DI_EUNSUPPORTED,
+             "%s: keys more than 2^22 elements apart", fn);
+  AttnEncArgs a = {};
+  a.q = pq.p, a.k = pk.p, a.v = pv.p, a.o = po.p;
+  a.ldq = pq.token, a.hq = pq.head, a.bq = pq.batch;
+  a.ldk = pk.token, a.hk = pk.head, a.bk = pk.batch;
+  a.ldv = pv.token, a.hv = pv.head, a.bv = pv.batch;
+  a.ldo = po.token, a.ho = po.head, a.bo = po.batch;
+  if (kv_len) {
+    DI_BUF(ctx, kv_len, lb, (uint64_t)B * 4);
+    DI_REQUIRE(kv_len != o->buf, DI_EINVAL, "%s: o overlaps kv_len", fn);
+    a.len = (const int32_t*)lb->ptr;
+  }
+  if (bias) {
+    DI_REQUIRE(bias->offset < kMaxStride && bias->batch < kMaxStride && bias->head < kMaxStride &&
+                   bias->query < kMaxStride,
+               DI_EINVAL, "%s: offset or stride of bias past 2^40 elements", fn);
+    Buffer* bb = nullptr;
+    rc = lookup(ctx, bias->buf, &bb);
+    if (rc) return rc;
+    const unsigned __int128 end = (unsigned __int128)bias->offset + (unsigned __int128)(B - 1) * bias->batch +
+                                  (unsigned __int128)(Hq - 1) * bias->head +
+                                  (unsigned __int128)(Sq - 1) * bias->query + Skv;
+    DI_REQUIRE(end * 4 <= bb->bytes, DI_EINVAL, "%s: bias ends past its buffer of %llu bytes", fn,
+               (unsigned long long)bb->bytes);
+    DI_REQUIRE(bias->buf != o->buf, DI_EINVAL, "%s: o overlaps bias", fn);
+    a.bias = (const float*)bb->ptr + bias->offset;
+    a.bias_b = bias->batch, a.bias_h = bias->head, a.bias_q = bias->query;
+  }
+  a.Hk = Hk, a.G = Hq / Hk, a.Sq = Sq, a.Skv = Skv, a.d = d;
+  a.scale_log2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float)d)) * kLog2E;
+  const uint64_t rows = (uint64_t)Sq * a.G;
+  a.prows = rows * B * Hk;
+  const bool f32 = dt == DI_F32;
+  const bool few = rows <= 16;
+  const AttnEncForm form = f32 ? attn_enc_form_f32(d, few) : attn_enc_form_f16(d, few);
+  const uint32_t R = form.rows, KT = form.tile, WK = form.groups;
+  const uint64_t blocks = (rows + R - 1) / R, groups = blocks * B * Hk;
+  DI_REQUIRE(rows < 1ull << 31 && groups < 1ull << 24, DI_EUNSUPPORTED, "%s: %llu rows per key head, %llu workgroups",
+             fn, (unsigned long long)rows, (unsigned long long)groups);
+  a.rows = (uint32_t)rows;
+  a.blocks = (uint32_t)blocks;
+  // key ranges: enough workgroups for two a CU, each of at least four tiles per key group
+  const uint64_t n_tiles = (Skv + KT - 1) / KT, most = n_tiles / (4 * WK);
+  uint64_t sp = 2ull * ctx->num_cus / groups;
+  sp = sp < most ? sp : most;
+  sp = sp < 64 ? sp : 64;
+  a.splits = sp < 2 ? 1 : (uint32_t)sp;
+  DI_HIP(hipSetDevice(ctx->device));
+  void* ws = nullptr;
+  uint64_t cap = 0;
+  if (a.splits > 1) {
+    const uint64_t ob = a.splits * a.prows * d * 4;
+    rc = pool_alloc(ctx, ob + a.splits * a.prows * 8, &ws, &cap);
+    if (rc) return rc;
+    a.part_o = (float*)ws;
+    a.part_ml = (float*)((char*)ws + ob);
+  }
+  if (f32) launch_attn_enc_f32(a, B, few, ctx->stream);
+  else launch_attn_enc_f16(a, B, few, ctx->stream);
+  if (ws) pool_release(ctx, ws, cap);
+  DI_LAUNCH_CHECK();
+  return DI_OK;
+}

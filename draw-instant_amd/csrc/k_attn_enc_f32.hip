@@ -1,0 +1,14 @@
+// k_attn_enc instantiations: fp32 tensors on the fp32 MFMA.
+#include "k_attn_enc.h"
+
+namespace di {
+
+void launch_attn_enc_f32(const AttnEncArgs& a, uint32_t B, bool few, hipStream_t s) {
+  launch_enc<float>(a, B, few, s);
+}
+
+AttnEncForm attn_enc_form_f32(uint32_t d, bool few) {
+  return few ? enc_form<float, true>(d) : enc_form<float, false>(d);
+}
+
+}  // namespace di

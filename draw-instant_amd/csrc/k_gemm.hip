@@ -1042,13 +1042,16 @@ void launch_gemm(GemmArgs g, int elem, int a_mode, int b_mode, int tile_cfg, hip
   } else if (big) {
     launch_conv3_big(g, s);
   } else if (fast) {
-    if (a_mode == A_DENSE && g.ln_rows && g.splits <= 1) gemm_fast_dense_ex(g, tile_cfg, s);
+    if (g.lo_t) gemm_fast_lora(g, tile_cfg, s);
+    else if (a_mode == A_DENSE && g.ln_rows && g.splits <= 1) gemm_fast_dense_ex(g, tile_cfg, s);
     else if (a_mode == A_DENSE && g.rstats) gemm_fast_dense_ex(g, tile_cfg, s);
     else if (a_mode == A_DENSE) gemm_fast_dense(g, tile_cfg, s);
     else gemm_fast_conv(g, tile_cfg, s);
   } else if (elem == DI_F32 && gemm_f32_ok(g, a_mode, b_mode)) {
     gemm_f32(g, a_mode, b_mode, tile_cfg, s);  // with its own split-K reducer
     return;
+  } else if (g.lo_t) {
+    gemm_slow_lora(g, elem, tile_cfg, s);
   } else {
     gemm_slow(g, elem, a_mode, b_mode, tile_cfg, s);
   }

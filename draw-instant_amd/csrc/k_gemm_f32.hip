@@ -353,7 +353,8 @@ struct ConvNchw {
 // buffer (48 KiB at 128 x 128): the next stage's global loads are in flight in
 // registers while this one is computed, and two workgroups per CU overlap one's
 // split-and-store phase with the other's MFMAs.
-template <int BM, int BN, int AM, int BMD, typename TB>
+// LORA: the k index goes on over (adapter of the tile, rank) as in k_gemm_kernel.h.
+template <int BM, int BN, int AM, int BMD, typename TB, bool LORA>
 __global__ __launch_bounds__(256, 2) void k_gemm_f32(GemmArgs g) {
   constexpr int TM = BM / 32, TN = BN / 32;  // 16-row fragments of a wave tile
   constexpr uint32_t PA = BM * 64, PB = BN * 64;
@@ -361,6 +362,7 @@ __global__ __launch_bounds__(256, 2) void k_gemm_f32(GemmArgs g) {
   static_assert((BM + BN) * kRawLd * 4 <= 3 * (PA + PB), "unsplit tiles fit the parts' planes");
   __shared__ __attribute__((aligned(16))) char smem[3 * (PA + PB)];
   char *sA = smem, *sB = smem + 3 * PA;
+  __shared__ LoraTile<LORA ? BM : 1> sLo;
 
   args_warm(g);
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -397,6 +399,39 @@ __global__ __launch_bounds__(256, 2) void k_gemm_f32(GemmArgs g) {
 #pragma unroll
     for (int b = 0; b < TN; b++) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+  // adapters: k index e runs on over (adapter of the tile, rank) after the last k
+  uint32_t lo_total = 0;
+  int32_t rid[LORA ? BM / 32 : 1];
+  if constexpr (LORA) {
+    if (split == 0) {
+      if (wave == 0) lora_tile<BM>(g, m0, sLo);
+#pragma unroll
+      for (int i = 0; i < BM / 32; i++) rid[i] = lora_id(g, m0 + (threadIdx.x >> 3) + 32 * i);
+      __syncthreads();
+      lo_total = (uint32_t)sLo.n * g.lo_ld;
+    }
+  }
+  auto load_lora = [&](uint32_t e0, F32Tile<BM>& ta, F32Tile<BN>& tb) {
+    const uint32_t e = e0 + (threadIdx.x & 7) * 4, slot = e / g.lo_ld, rr = e - slot * g.lo_ld;
+    const int32_t ad = slot < (uint32_t)sLo.n ? sLo.ad[slot] : -2;
+#pragma unroll
+    for (int i = 0; i < BM / 32; i++) {
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      if (rid[i] == ad)
+        v = *(const f32x4*)((const float*)g.lo_t + (uint64_t)(m0 + (threadIdx.x >> 3) + 32 * i) * g.lo_ld + rr);
+#pragma unroll
+      for (int j = 0; j < 4; j++) ta.v[4 * i + j] = v[j];
+    }
+#pragma unroll
+    for (int i = 0; i < BN / 32; i++) {
+      const uint32_t n = n0 + (threadIdx.x >> 3) + 32 * i;
+      const bool ok = ad >= 0 && n < g.N;
+      const float* p = (const float*)g.lo_up + ((uint64_t)(ok ? ad : 0) * g.N + (ok ? n : 0)) * g.lo_rank + rr;
+#pragma unroll
+      for (int j = 0; j < 4; j++) tb.v[4 * i + j] = ok && rr + j < g.lo_rank ? p[j] : 0.0f;
+    }
+  };
+
   // D = mma(X, Y): a lane holds four consecutive X rows of one Y row, so X is
   // the operand whose index is contiguous in the output: A (pixels) for an
   // NCHW image, B (columns) otherwise.
@@ -410,17 +445,20 @@ __global__ __launch_bounds__(256, 2) void k_gemm_f32(GemmArgs g) {
     auto LB = make_b();
     F32Tile<BM> ta;
     F32Tile<BN> tb;
-    if (n_stages > 0) {
-      LA.load(k_begin, ta);
-      LB.load(k_begin, tb);
-    }
-    for (uint32_t s = 0; s < n_stages; s++) {
+    const uint32_t n_all = n_stages + (LORA ? (lo_total + 31) / 32 : 0u);
+    auto load = [&](uint32_t s) {
+      if (LORA && s >= n_stages) {
+        load_lora((s - n_stages) * 32, ta, tb);
+        return;
+      }
+      LA.load(k_begin + s * 32, ta);
+      LB.load(k_begin + s * 32, tb);
+    };
+    if (n_all > 0) load(0);
+    for (uint32_t s = 0; s < n_all; s++) {
       store_split<float>(sA, ta, A_KMAJ);
       store_split<TB>(sB, tb, B_KMAJ);
-      if (s + 1 < n_stages) {  // on its way while this stage is computed
-        LA.load(k_begin + (s + 1) * 32, ta);
-        LB.load(k_begin + (s + 1) * 32, tb);
-      }
+      if (s + 1 < n_all) load(s + 1);  // on its way while this stage is computed
       lds_barrier();
       bf16x8 bf[TN][3];
 #pragma unroll
@@ -461,11 +499,15 @@ __global__ __launch_bounds__(256, 2) void k_gemm_f32(GemmArgs g) {
     for (int a = 0; a < TM; a++)
 #pragma unroll
       for (int b = 0; b < TN; b++) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (uint32_t s = 0; s < n_stages; s++) {
+    for (uint32_t s = 0; s < n_stages + (LORA ? (lo_total + 31) / 32 : 0u); s++) {
       F32Tile<BM> ta;
       F32Tile<BN> tb;
-      LA.load(k_begin + s * 32, ta);
-      LB.load(k_begin + s * 32, tb);
+      if (LORA && s >= n_stages) {
+        load_lora((s - n_stages) * 32, ta, tb);
+      } else {
+        LA.load(k_begin + s * 32, ta);
+        LB.load(k_begin + s * 32, tb);
+      }
       __syncthreads();
       store_raw(fA, ta, A_KMAJ);
       store_raw(fB, tb, B_KMAJ);
@@ -650,17 +692,17 @@ __global__ __launch_bounds__(256) void k_f32_reduce(GemmArgs g) {
   }
 }
 
-template <int BM, int BN, int AM, int BMD, typename TB>
+template <int BM, int BN, int AM, int BMD, typename TB, bool LORA>
 void launch_f32_tile(const GemmArgs& g, hipStream_t s) {
   const dim3 grid(((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN), 1, g.batch * g.splits);
-  k_gemm_f32<BM, BN, AM, BMD, TB><<<grid, 256, 0, s>>>(g);
+  k_gemm_f32<BM, BN, AM, BMD, TB, LORA><<<grid, 256, 0, s>>>(g);
 }
 
-template <int AM, int BMD, typename TB>
+template <int AM, int BMD, typename TB, bool LORA = false>
 void launch_f32(const GemmArgs& g, int tile, hipStream_t s) {
-  if (tile == TILE_128x128) launch_f32_tile<128, 128, AM, BMD, TB>(g, s);
-  else if (tile == TILE_128x64) launch_f32_tile<128, 64, AM, BMD, TB>(g, s);
-  else launch_f32_tile<64, 64, AM, BMD, TB>(g, s);
+  if (tile == TILE_128x128) launch_f32_tile<128, 128, AM, BMD, TB, LORA>(g, s);
+  else if (tile == TILE_128x64) launch_f32_tile<128, 64, AM, BMD, TB, LORA>(g, s);
+  else launch_f32_tile<64, 64, AM, BMD, TB, LORA>(g, s);
 }
 
 }  // namespace
@@ -692,7 +734,8 @@ void gemm_f32(const GemmArgs& g, int a_mode, int b_mode, int tile, hipStream_t s
     if (g.b_f16) launch_f32<A_CONV_NCHW, B_NK, f16>(g, tile, s);
     else launch_f32<A_CONV_NCHW, B_NK, float>(g, tile, s);
   } else if (b_mode == B_NK) {
-    if (g.b_f16) launch_f32<A_DENSE, B_NK, f16>(g, tile, s);
+    if (g.lo_t) launch_f32<A_DENSE, B_NK, float, true>(g, tile, s);
+    else if (g.b_f16) launch_f32<A_DENSE, B_NK, f16>(g, tile, s);
     else launch_f32<A_DENSE, B_NK, float>(g, tile, s);
   } else {
     if (g.b_f16) launch_f32<A_DENSE, B_KN, f16>(g, tile, s);

@@ -13,6 +13,11 @@ void gemm_fast_dense(const GemmArgs& g, int tile_cfg, hipStream_t s);
 // The same path with an epilogue extra: the LayerNorm fold (g.ln_rows, no
 // split) or the output row statistics (g.rstats) (k_gemm_dense_ex.hip).
 void gemm_fast_dense_ex(const GemmArgs& g, int tile_cfg, hipStream_t s);
+// Dense A with low-rank adapters (g.lo_t): the buffer-load path and the
+// bounds-checked kernels (k_gemm_dense_lora.hip); fp32 goes to gemm_f32 where
+// that takes the problem.
+void gemm_fast_lora(const GemmArgs& g, int tile_cfg, hipStream_t s);
+void gemm_slow_lora(const GemmArgs& g, int elem, int tile_cfg, hipStream_t s);
 // fp16 buffer-load path, implicit-GEMM NHWC conv (k_gemm_conv.hip).
 void gemm_fast_conv(const GemmArgs& g, int tile_cfg, hipStream_t s);
 // fp32 on the bf16 matrix cores with split operands and its split-K reducer

@@ -223,9 +223,49 @@ __device__ __forceinline__ void epi_math8(const GemmArgs& g, float* x, const f32
 
 // Epilogue extras of the dense buffer-load kernels (template parameter EX):
 // EX_ROWSTATS writes g.rstats, EX_LNFOLD applies the LayerNorm fold of
-// g.ln_*.  Separate instantiations keep their registers out of every other
+// g.ln_*; EX_LORA (any kernel with dense A and B_NK) adds the adapters' product
+// (g.lo_*) as further k stages.  Separate instantiations keep their registers out of every other
 // GEMM's allocation.
-enum { EX_NONE = 0, EX_ROWSTATS = 1, EX_LNFOLD = 2 };
+enum { EX_NONE = 0, EX_ROWSTATS = 1, EX_LNFOLD = 2, EX_LORA = 3 };
+
+// The adapters that a tile's rows name (g.lo_*), each once, in order of first
+// appearance: `n` of them.
+template <int BM>
+struct LoraTile {
+  int32_t ad[BM];
+  int32_t n;
+};
+
+// Adapter of row m, -1 where it has none.
+__device__ __forceinline__ int32_t lora_id(const GemmArgs& g, uint32_t m) {
+  if (m >= g.M) return -1;
+  const int32_t id = g.lo_ids[m / g.lo_run];
+  return (uint32_t)id < g.lo_n ? id : -1;
+}
+
+// Fills `lo` for rows m0 .. m0 + BM - 1: one wavefront, no barrier.
+template <int BM>
+__device__ __forceinline__ void lora_tile(const GemmArgs& g, uint32_t m0, LoraTile<BM>& lo) {
+  constexpr int NI = (BM + 63) / 64;
+  const uint32_t lane = threadIdx.x & 63;
+  int32_t id[NI];
+#pragma unroll
+  for (int i = 0; i < NI; i++) id[i] = lane + 64 * i < BM ? lora_id(g, m0 + lane + 64 * i) : -1;
+  int32_t n = 0;
+#pragma unroll
+  for (int i = 0; i < NI; i++) {
+    uint64_t todo;
+    while ((todo = __builtin_amdgcn_ballot_w64(id[i] >= 0)) != 0) {
+      const int32_t a = __builtin_amdgcn_readlane(id[i], __builtin_ctzll(todo));
+      if (lane == 0) lo.ad[n] = a;
+      n++;
+#pragma unroll
+      for (int k = i; k < NI; k++)
+        if (id[k] == a) id[k] = -1;
+    }
+  }
+  if (lane == 0) lo.n = n;
+}
 
 // Barrier for hand-offs through LDS inside a workgroup: waits for the
 // wave's LDS operations only and meets the other waves, leaving global
@@ -586,7 +626,8 @@ __device__ __forceinline__ void args_warm(const GemmArgs& g) { kernarg_warm(g); 
 template <typename T, int BM, int BN, int WGM, int WGN, int AM, int BMD, bool FAST, int D, int KS,
           int EX, typename TB = T>
 __global__ __launch_bounds__(64 * WGM * WGN * KS) void k_gemm(GemmArgs g) {
-  static_assert(EX == EX_NONE || (FAST && AM == A_DENSE), "epilogue extras: dense fast path");
+  static_assert(EX == EX_NONE || (AM == A_DENSE && (FAST || (EX == EX_LORA && BMD == B_NK))),
+                "epilogue extras: dense fast path (adapters: any dense path)");
   static_assert(std::is_same<TB, T>::value || (!FAST && std::is_same<T, float>::value &&
                                                std::is_same<TB, f16>::value),
                 "fp16 B with fp32 A: bounds-checked fp32 kernels only");
@@ -637,6 +678,7 @@ __global__ __launch_bounds__(64 * WGM * WGN * KS) void k_gemm(GemmArgs g) {
   __shared__ __attribute__((aligned(16))) T smem[SBS ? kSmem2 : kSmem1];
   // LayerNorm fold: (mean, rstd) of each tile row, then ln_s of each column
   __shared__ __attribute__((aligned(16))) float sLn[EX == EX_LNFOLD ? 2 * BM + BN : 2];
+  __shared__ LoraTile<EX == EX_LORA ? BM : 1> sLo;
   T (*sA)[BM * LDK] = reinterpret_cast<T (*)[BM * LDK]>(smem);
   T (*sB)[BN * LDK] = reinterpret_cast<T (*)[BN * LDK]>(smem + 2 * BM * LDK);
   // element offset of (row r, k element e) inside one buffer
@@ -1067,6 +1109,54 @@ __global__ __launch_bounds__(64 * WGM * WGN * KS) void k_gemm(GemmArgs g) {
   }
   }
 
+  // Adapters: the tile's k index goes on over (adapter of the tile, rank), the
+  // A operand being the row's own inner products lo_t under its own adapter
+  // and zero under the others; a stage may hold several adapters.  One split
+  // takes them.
+  if constexpr (EX == EX_LORA) {
+    if (split == 0) {
+      if (wave == 0) lora_tile<BM>(g, m0, sLo);
+      int32_t rid[NVA];
+#pragma unroll
+      for (int i = 0; i < NVA; i++) rid[i] = a_ld ? lora_id(g, m0 + (tid + i * NT) / VPR) : -1;
+      __syncthreads();
+      const int32_t n_ad = sLo.n;
+      const uint32_t total = (uint32_t)n_ad * g.lo_ld;
+      const bool whole = g.lo_rank == g.lo_ld;
+      for (uint32_t e0 = 0; e0 < total; e0 += BK) {
+        const uint32_t e = e0 + kc * KV, slot = e / g.lo_ld, rr = e - slot * g.lo_ld;
+        const int32_t ad = slot < (uint32_t)n_ad ? sLo.ad[slot] : -2;
+        Stage st;
+#pragma unroll
+        for (int i = 0; i < NVA; i++) {
+          st.a[i] = zero_vec<T>();
+          if (rid[i] == ad)
+            st.a[i] = *(const typename MT::vec*)((const T*)g.lo_t +
+                                                 (uint64_t)(m0 + (tid + i * NT) / VPR) * g.lo_ld + rr);
+        }
+#pragma unroll
+        for (int i = 0; i < NVB; i++) {
+          st.b[i] = zero_vec<T>();
+          const uint32_t n = n0 + (tid + i * NT) / VPR;
+          if (b_ld && ad >= 0 && n < g.N) {
+            const T* p = (const T*)g.lo_up + ((uint64_t)ad * g.N + n) * g.lo_rank + rr;
+            if (whole) {
+              st.b[i] = *(const typename MT::vec*)p;
+            } else {
+#pragma unroll
+              for (int j = 0; j < KV; j++)
+                if (rr + j < g.lo_rank) st.b[i][j] = p[j];
+            }
+          }
+        }
+        store_stage(0, st);
+        __syncthreads();
+        compute(0);
+        __syncthreads();
+      }
+    }
+  }
+
   // ---- epilogue ----
   const uint32_t rq = (lane >> 4) * 4;
   if constexpr (sizeof(T) == 2) {
@@ -1219,22 +1309,22 @@ void launch_cfg(const GemmArgs& g, hipStream_t s) {
 // Generic (bounds-checked) variants: two tile shapes.  fp32 takes the larger one only where 64 x 64 tiles
 // would pass the grid's 2^32 threads (128 -> 3 channels at 1536 x 1536: 6.8 ms on
 // 64 x 64, 16.1 on 128 x 128; 128 -> 128 13.8 and 17.3).
-template <typename T, int AM, int BMD, typename TB = T>
+template <typename T, int AM, int BMD, typename TB = T, int EX = EX_NONE>
 void launch_slow(const GemmArgs& g, int tile_cfg, hipStream_t s) {
   if constexpr (sizeof(T) == 4) {
     const uint64_t tiles = (uint64_t)((g.M + 63) / 64) * ((g.N + 63) / 64);
     if (tiles * 256 < (1ull << 32))
-      launch_cfg<T, 64, 64, 2, 2, AM, BMD, false, 2, 1, EX_NONE, TB>(g, s);
+      launch_cfg<T, 64, 64, 2, 2, AM, BMD, false, 2, 1, EX, TB>(g, s);
     else
-      launch_cfg<T, 128, 128, 2, 2, AM, BMD, false, 2, 1, EX_NONE, TB>(g, s);
+      launch_cfg<T, 128, 128, 2, 2, AM, BMD, false, 2, 1, EX, TB>(g, s);
     return;
   } else if (tile_cfg == TILE_64x64 || tile_cfg == TILE_128x64 || tile_cfg == TILE_64x128 ||
       tile_cfg == TILE_64x160 || tile_cfg == TILE_64x64_K2 || tile_cfg == TILE_128x64_K2 ||
       tile_cfg == TILE_64x128_K2 || tile_cfg == TILE_64x128_W16 || tile_cfg == TILE_128x64_W16 ||
       tile_cfg == TILE_64x64_W16)
-    launch_cfg<T, 64, 64, 2, 2, AM, BMD, false, 2, 1, EX_NONE, TB>(g, s);
+    launch_cfg<T, 64, 64, 2, 2, AM, BMD, false, 2, 1, EX, TB>(g, s);
   else
-    launch_cfg<T, 128, 128, 2, 2, AM, BMD, false, 2, 1, EX_NONE, TB>(g, s);
+    launch_cfg<T, 128, 128, 2, 2, AM, BMD, false, 2, 1, EX, TB>(g, s);
 }
 
 // Buffer-load variants: every tile shape, ring depth D, epilogue extras EX.

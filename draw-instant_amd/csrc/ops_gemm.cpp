@@ -72,6 +72,46 @@ struct Tmp {
   }
 };
 
+
+// The arguments of a linear in torch layout after its checks.
+int linear_args(di_ctx* ctx, const char* fn, di_handle X, di_handle W, di_handle bias, di_handle R, di_handle Y,
+                uint32_t M, uint32_t N, uint32_t K, int32_t act, int32_t dt, GemmArgs& g) {
+  DI_REQUIRE(M && N && K, DI_EINVAL, "%s: zero dimension (M=%u N=%u K=%u)", fn, M, N, K);
+  DI_REQUIRE(act >= ACT_NONE && act <= ACT_GELU_TANH, DI_EINVAL, "%s: unknown act %d", fn, act);
+  DI_REQUIRE(act != ACT_GEGLU || N % 32 == 0, DI_EINVAL, "%s: GEGLU needs N %% 32 == 0 (got %u)", fn, N);
+  const size_t es = dtype_size(dt);
+  const uint32_t nout = act == ACT_GEGLU ? N / 2 : N;
+  DI_BUF(ctx, X, x, (uint64_t)M * K * es);
+  DI_BUF(ctx, W, w, (uint64_t)N * K * es);
+  DI_BUF(ctx, Y, y, (uint64_t)M * nout * es);
+  const float* b = nullptr;
+  int rc = opt_f32(ctx, bias, N, &b);
+  if (rc) return rc;
+  if (R) {
+    DI_BUF(ctx, R, r, (uint64_t)M * nout * es);
+    g.res = r->ptr;
+    g.ldr = nout;
+    g.res_f32 = dt == DI_F32;
+  }
+  g.a = x->ptr;
+  g.lda = K;
+  g.b = w->ptr;
+  g.ldb = K;
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.bias = b;
+  g.act = act;
+  g.c = y->ptr;
+  g.ldc = nout;
+  g.c_f32 = dt == DI_F32;
+  const uint32_t kv = dt == DI_F32 ? 4 : 8;
+  g.a_vec_ok = g.b_vec_ok = K % kv == 0;
+  g.a_bytes = gemm_extent((uint64_t)M * K * es);
+  g.b_bytes = gemm_extent((uint64_t)N * K * es);
+  return DI_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -149,41 +189,53 @@ int32_t di_linear(di_ctx* ctx, di_handle X, di_handle W, di_handle bias, di_hand
                   uint32_t M, uint32_t N, uint32_t K, int32_t act, int32_t dt) {
   DI_CTX(ctx);
   DI_DTYPE(dt);
-  DI_REQUIRE(M && N && K, DI_EINVAL, "di_linear: zero dimension (M=%u N=%u K=%u)", M, N, K);
-  DI_REQUIRE(act >= ACT_NONE && act <= ACT_GELU_TANH, DI_EINVAL, "di_linear: unknown act %d", act);
-  DI_REQUIRE(act != ACT_GEGLU || N % 32 == 0, DI_EINVAL,
-             "di_linear: GEGLU needs N %% 32 == 0 (got %u)", N);
-  const size_t es = dtype_size(dt);
-  const uint32_t nout = act == ACT_GEGLU ? N / 2 : N;
-  DI_BUF(ctx, X, x, (uint64_t)M * K * es);
-  DI_BUF(ctx, W, w, (uint64_t)N * K * es);
-  DI_BUF(ctx, Y, y, (uint64_t)M * nout * es);
-  const float* b = nullptr;
-  int rc = opt_f32(ctx, bias, N, &b);
-  if (rc) return rc;
   GemmArgs g;
-  if (R) {
-    DI_BUF(ctx, R, r, (uint64_t)M * nout * es);
-    g.res = r->ptr;
-    g.ldr = nout;
-    g.res_f32 = dt == DI_F32;
-  }
-  g.a = x->ptr;
-  g.lda = K;
-  g.b = w->ptr;
-  g.ldb = K;
-  g.M = M;
-  g.N = N;
-  g.K = K;
-  g.bias = b;
-  g.act = act;
-  g.c = y->ptr;
-  g.ldc = nout;
-  g.c_f32 = dt == DI_F32;
+  const int rc = linear_args(ctx, "di_linear", X, W, bias, R, Y, M, N, K, act, dt, g);
+  if (rc) return rc;
+  return run_gemm(ctx, g, dt, A_DENSE, B_NK);
+}
+
+int32_t di_linear_lora(di_ctx* ctx, di_handle X, di_handle W, di_handle bias, const di_lora* lora,
+                       di_handle R, di_handle Y, uint32_t M, uint32_t N, uint32_t K, int32_t act,
+                       int32_t dt) {
+  const char* fn = "di_linear_lora";
+  DI_REQUIRE(ctx != nullptr, DI_EINVAL, "null context");
+  DI_DTYPE(dt);
+  DI_REQUIRE(lora != nullptr, DI_EINVAL, "%s: null adapters", fn);
+  GemmArgs g;
+  int rc = linear_args(ctx, fn, X, W, bias, R, Y, M, N, K, act, dt, g);
+  if (rc) return rc;
+  DI_REQUIRE(Y != X && Y != W, DI_EINVAL, "%s: Y is an operand", fn);
+  DI_REQUIRE(lora->n && lora->rank && lora->rows_per_id, DI_EINVAL, "%s: zero dimension (n=%u rank=%u rows_per_id=%u)",
+             fn, lora->n, lora->rank, lora->rows_per_id);
+  DI_REQUIRE(lora->rank <= 256, DI_EUNSUPPORTED, "%s: rank %u above 256", fn, lora->rank);
+  DI_REQUIRE(lora->n < 1u << 31, DI_EINVAL, "%s: %u adapters", fn, lora->n);
+  const size_t es = dtype_size(dt);
+  const uint64_t nr = (uint64_t)lora->n * lora->rank;
+  DI_REQUIRE((unsigned __int128)nr * (N > K ? N : K) < 1ull << 60, DI_EINVAL, "%s: stack too large", fn);
+  DI_BUF(ctx, lora->down, down, nr * K * es);
+  DI_BUF(ctx, lora->up, up, nr * N * es);
+  DI_BUF(ctx, lora->ids, ids, ((uint64_t)M + lora->rows_per_id - 1) / lora->rows_per_id * 4);
+  const float* scale = nullptr;
+  rc = opt_f32(ctx, lora->scale, lora->n, &scale);
+  if (rc) return rc;
+  DI_REQUIRE(Y != lora->down && Y != lora->up && Y != lora->ids && (!scale || Y != lora->scale), DI_EINVAL,
+             "%s: Y is an operand", fn);
   const uint32_t kv = dt == DI_F32 ? 4 : 8;
-  g.a_vec_ok = g.b_vec_ok = K % kv == 0;
-  g.a_bytes = gemm_extent((uint64_t)M * K * es);
-  g.b_bytes = gemm_extent((uint64_t)N * K * es);
+  g.lo_up = up->ptr;
+  g.lo_ids = (const int32_t*)ids->ptr;
+  g.lo_n = lora->n;
+  g.lo_rank = lora->rank;
+  g.lo_ld = (lora->rank + kv - 1) / kv * kv;
+  g.lo_run = lora->rows_per_id;
+  DI_HIP(hipSetDevice(ctx->device));
+  Tmp t(ctx);
+  rc = t.alloc((uint64_t)M * g.lo_ld * es);
+  if (rc) return rc;
+  g.lo_t = t.p;
+  launch_lora_down(g.a, down->ptr, scale, g.lo_ids, t.p, M, K, g.lo_n, g.lo_rank, g.lo_ld, g.lo_run, dt,
+                   ctx->num_cus, ctx->stream);
+  DI_LAUNCH_CHECK();
   return run_gemm(ctx, g, dt, A_DENSE, B_NK);
 }
 

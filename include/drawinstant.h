@@ -272,6 +272,26 @@ int32_t di_gemm(di_ctx* ctx, di_handle A, di_handle B, di_handle C, di_handle Y,
 int32_t di_linear(di_ctx* ctx, di_handle X, di_handle W, di_handle bias, di_handle R,
                   di_handle Y, uint32_t M, uint32_t N, uint32_t K, int32_t act,
                   int32_t dtype);
+/* Low-rank adapters of many requests beside a shared projection (no reference
+ * counterpart: the reference's weights are fixed).  A stack of n adapters of
+ * one rank: down [n][rank][K] and up [n][N][rank] of the call's dtype (smaller
+ * ranks padded with zeros), scale fp32 [n] (0 handle: all 1).  ids: int32
+ * [ceil(M / rows_per_id)], the adapter of each run of rows_per_id rows, in any
+ * order; an id outside [0, n) (-1) leaves its rows without one. */
+typedef struct {
+  di_handle down, up, scale, ids;
+  uint32_t n, rank, rows_per_id;
+} di_lora;
+/* di_linear with adapters: row m, a = ids[m / rows_per_id],
+ * Y = act(X W^T + bias + scale[a] (X down[a]^T) up[a]^T) + R.
+ * rank 1 to 256; with DI_ACT_GEGLU the rows of up are interleaved as W's.
+ * The scaled inner products X down^T are held in dtype between the two
+ * products, as activations are; every sum is fp32.  The stack must be finite:
+ * rows of one tile are multiplied with each other's adapters by zeros.  Y may
+ * be R, not X. */
+int32_t di_linear_lora(di_ctx* ctx, di_handle X, di_handle W, di_handle bias,
+                       const di_lora* lora, di_handle R, di_handle Y, uint32_t M, uint32_t N,
+                       uint32_t K, int32_t act, int32_t dtype);
 /* Conv2d, square kernel K, stride S, symmetric pad (convMM wgsl-ops.js:584-711,
  * OPS.Conv wgsl-executor.js:1068-1092; batch N >= 1, the reference computes
  * batch 0 only).  Optional residual R (same shape as Y) added after the bias
@@ -301,6 +321,76 @@ int32_t di_attn_self(di_ctx* ctx, di_handle Q, di_handle K, di_handle V, di_hand
 int32_t di_attn_cross(di_ctx* ctx, di_handle Q, di_handle K, di_handle V, di_handle O,
                       uint32_t B, uint32_t H, uint32_t Sq, uint32_t Skv, uint32_t d,
                       int32_t layout, float scale, int32_t dtype);
+
+/* A view of heads in a buffer: element (b, s, h, c) of [B][S][H][d] lies at
+ * offset + b * batch + s * token + h * head + c, in elements.  Covers both
+ * attention layouts, the parts of a stacked projection, a run of tokens in a
+ * longer sequence (offset), and for inputs one sequence for a whole batch
+ * (batch stride 0). */
+typedef struct {
+  di_handle buf;
+  uint64_t offset, token, head, batch;
+} di_heads;
+
+/* ---- di_qk_norm_rope: norms and pairings ---- */
+#define DI_QKN_NONE 0 /* no norm: the rotation alone */
+#define DI_QKN_RMS 1  /* x / sqrt(mean(x^2) + eps) * gamma over each head's d channels */
+#define DI_ROPE_HALVES 1       /* channel p pairs with p + r/2 (r rotated channels); else 2p with 2p + 1 */
+#define DI_ROPE_ONE_SPECTRUM 2 /* pair p turns by theta[0]^(-2p/r) whatever its axis; else each
+                                  axis has its own: theta[a]^(-2i/dim[a]) for its i-th pair */
+
+/* Rotation by positions of several axes (time, height, width): the first
+ * r = dim[0] + dim[1] + ... channels of a head are rotated in pairs, dim[a] / 2
+ * pairs per axis in order, the rest passes.  Pair (u, w) at position t:
+ * (u cos - w sin, w cos + u sin) of the angle t * frequency.  axes = 0: no
+ * rotation.  Positions: fp32 [S][axes] per batch entry, pos_batch elements
+ * apart (0: one set for the batch). */
+typedef struct {
+  uint32_t axes;   /* 0 to 4 */
+  uint32_t dim[4]; /* even, their sum at most d */
+  float theta[4];  /* > 1 */
+  uint32_t flags;
+  uint64_t pos_batch;
+} di_rope;
+
+/* Norm of each query and key head and its rotation in one pass (no reference
+ * counterpart: the SD U-Net has neither).  q, q_out: Hq heads; k, k_out: Hk
+ * heads (both null: queries only).  q_gamma / k_gamma: fp32 [d], 0 = ones.
+ * d at most 256, of any alignment.  An output view may be its own input view
+ * (in place); otherwise no output may overlap an input or the other output.
+ * Angles are formed in 64 bits, the rest in fp32, rounded once. */
+int32_t di_qk_norm_rope(di_ctx* ctx, const di_heads* q, const di_heads* k,
+                        const di_heads* q_out, const di_heads* k_out, di_handle q_gamma,
+                        di_handle k_gamma, di_handle pos, const di_rope* rope, uint32_t B,
+                        uint32_t S, uint32_t Hq, uint32_t Hk, uint32_t d, int32_t norm,
+                        float eps, int32_t dtype);
+
+/* An additive score bias: fp32, element (b, h, i, j) of query i and key j of
+ * query head h at offset + b * batch + h * head + i * query + j; strides of 0
+ * broadcast. */
+typedef struct {
+  di_handle buf;
+  uint64_t offset, batch, head, query;
+} di_attn_bias;
+
+/* Attention to an encoder's states of another length: the general form of
+ * di_attn_cross (fused-cross-attn.js:112-173).  o = softmax(scale q k^T + bias) v
+ * for q, o [B][Sq][Hq][d] and k, v [B][Skv][Hk][d]; query head h reads key
+ * head h / (Hq / Hk) (Hk divides Hq).  d: a multiple of 8 up to 256; every
+ * offset and stride of the views a multiple of 8 elements.
+ *   kv_len (0 = none): int32 [B] on the device, the keys of each batch entry,
+ *     clamped to [0, Skv]; what lies behind them is never read.
+ *   bias (null = none): finite values or -inf.  -inf removes a key: its K may
+ *     hold anything, and its V too where no query of the call sees it.  A
+ *     finite bias of -1e30 or below replaces the score.
+ * A query with no key left gets zeros.  scale <= 0 selects 1/sqrt(d).  fp16
+ * runs on the fp16 MFMA (probabilities and scale * q rounded to fp16), fp32
+ * on the fp32 MFMA; maxima, sums and outputs accumulate in fp32.  o may not
+ * overlap k, v or q. */
+int32_t di_attn_encoder(di_ctx* ctx, const di_heads* q, const di_heads* k, const di_heads* v,
+                        const di_heads* o, di_handle kv_len, const di_attn_bias* bias,
+                        uint32_t B, uint32_t Hq, uint32_t Hk, uint32_t Sq, uint32_t Skv,
+                        uint32_t d, float scale, int32_t dtype);
 
 /* ======================= timestep embedding ======================= */
 
