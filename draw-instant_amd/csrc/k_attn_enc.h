@@ -8,9 +8,11 @@
 // row = query * G + head, so that one read of a key serves all of them, and a
 // single token's heads fill a 16-row MFMA tile together.
 //
-// MFMA mapping, as in k_attn.hip: S^T = K Q'^T with Q' = q * scale * log2(e)
-// (in the tensors' type), so scores come out in log2 units with the C layout
-// leaving lane l row l%16 and keys 4g..4g+3 (g = l/16) of each 16-key tile;
+// MFMA mapping, as in k_attn.hip: S^T = K Q^T, the C layout leaving lane l row
+// l%16 and keys 4g..4g+3 (g = l/16) of each 16-key tile; scale * log2(e) comes
+// in with the maximum, one fma before the exp2 (folded into Q it would cost no
+// instruction less here and round fp16 queries a second time: 4.3e-4 instead of
+// 3.0e-4 off 64 bits at 512 keys);
 // O^T += V^T P^T takes those probabilities as its B operand without moving
 // them.  fp16: v_mfma_f32_16x16x32_f16, the V^T operand by transposed LDS
 // reads.  fp32: v_mfma_f32_16x16x4_f32 on four registers of a 16-byte read,
@@ -172,10 +174,8 @@ void k_attn_enc(AttnEncArgs a) {
 #pragma unroll
     for (int c = 0; c < QC; c++) {
       const uint32_t e = (c * 4 + g) * EPC;
-      frag t = {};
-      if (live[i] && e < a.d) t = *(const frag*)(p + e);
-#pragma unroll
-      for (int j = 0; j < EPC; j++) qf[i][c][j] = (T)((float)t[j] * a.scale_log2);
+      qf[i][c] = frag{};
+      if (live[i] && e < a.d) qf[i][c] = *(const frag*)(p + e);
     }
   }
   const float* bp[QG];
@@ -322,9 +322,10 @@ void k_attn_enc(AttnEncArgs a) {
               bb[i][kt][j] = x == -INFINITY ? x : fmaxf(x * kLog2E, kLowest);
             }
       }
+      // in log2 units
       auto score = [&](int i, int kt, int j) -> float {
-        if constexpr (BIAS) return s[i][kt][j] + bb[i][kt][j];
-        else return s[i][kt][j];
+        if constexpr (BIAS) return fmaf(s[i][kt][j], a.scale_log2, bb[i][kt][j]);
+        else return s[i][kt][j] * a.scale_log2;
       };
       // raise the running maximum to this tile's where that is larger
       auto raise = [&](int i) {
@@ -348,7 +349,7 @@ void k_attn_enc(AttnEncArgs a) {
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             // with a bias, (bias - m) first: it is exact where they are close
-            const float x = BIAS ? s[i][kt][j] + (bb[i][kt][j] - m[i]) : s[i][kt][j] - m[i];
+            const float x = fmaf(s[i][kt][j], a.scale_log2, BIAS ? bb[i][kt][j] - m[i] : -m[i]);
             pr[i][kt][j] = __builtin_amdgcn_exp2f(x);
             ts[i] += pr[i][kt][j];
           }

@@ -384,8 +384,8 @@ typedef struct {
  *     hold anything, and its V too where no query of the call sees it.  A
  *     finite bias of -1e30 or below replaces the score.
  * A query with no key left gets zeros.  scale <= 0 selects 1/sqrt(d).  fp16
- * runs on the fp16 MFMA (probabilities and scale * q rounded to fp16), fp32
- * on the fp32 MFMA; maxima, sums and outputs accumulate in fp32.  o may not
+ * runs on the fp16 MFMA (probabilities rounded to fp16), fp32 on the fp32
+ * MFMA; scores, maxima, sums and outputs accumulate in fp32.  o may not
  * overlap k, v or q. */
 int32_t di_attn_encoder(di_ctx* ctx, const di_heads* q, const di_heads* k, const di_heads* v,
                         const di_heads* o, di_handle kv_len, const di_attn_bias* bias,
