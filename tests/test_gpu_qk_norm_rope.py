@@ -127,3 +127,21 @@ def test_small_values(dev, rng):
     check(got, y, bound, "small")
     for t in (b, p, o):
         t.destroy()
+
+
+@pytest.mark.parametrize("halves", [False, True])
+def test_infinite_channels_that_do_not_turn(dev, rng, halves):
+    """Without a norm the channels past the rotated ones pass whatever they hold."""
+    from drawinstant import attention as at
+    x = rng.standard_normal((1, 6, 2, 24)).astype(F32)
+    x[0, :, 0, 20] = np.inf
+    x[0, 1, 1, 17:] = np.nan
+    b, p, o = dev.storage(x), dev.storage(np.arange(6, dtype=F32)), dev.create_buffer(x.nbytes)
+    at.qk_norm_rope(dev, at.heads(b, 6, 2, 24), None, at.heads(o, 6, 2, 24), None, p, at.Rope([16], halves=halves),
+                    1, 6, 2, 0, 24, norm=at.NORM_NONE, dtype=0)
+    got = dev.download(o, F32, x.shape)
+    assert np.array_equal(got[..., 16:], x[..., 16:], equal_nan=True)
+    y, bound = qk(x[..., :16], None, np.arange(6).reshape(1, 6, 1), [16], [1e4], halves, False, 0, 0, F32)
+    check(got[..., :16], y, bound, "rotated part")
+    for t in (b, p, o):
+        t.destroy()
