@@ -27,15 +27,19 @@ struct AttnEncArgs {
   float* part_ml;  // [splits][prows][2]
 };
 
-// f32: tensors and matrix products in fp32 (k_attn_enc_f32.hip), else fp16.
-void launch_attn_enc_f16(const AttnEncArgs& a, uint32_t B, bool few, hipStream_t s);
-void launch_attn_enc_f32(const AttnEncArgs& a, uint32_t B, bool few, hipStream_t s);
-// Rows per workgroup, keys per tile and key groups inside a workgroup of the
-// form for few or many rows (see k_attn_enc.h).
+// The three forms (see k_attn_enc.h): rows per workgroup, keys per tile and key
+// groups inside a workgroup.
+enum { ENC_FEW = 0, ENC_MID = 1, ENC_MANY = 2 };
+// Whether a form is built with a bias: two row groups with one and over 64
+// channels do not fit the registers (154 spilled at 128).
+constexpr bool enc_bias_ok(uint32_t d, int form) { return form != ENC_MANY || d <= 64; }
 struct AttnEncForm {
   int rows, tile, groups;
 };
-AttnEncForm attn_enc_form_f16(uint32_t d, bool few);
-AttnEncForm attn_enc_form_f32(uint32_t d, bool few);
+AttnEncForm attn_enc_form_f16(uint32_t d, int form);
+AttnEncForm attn_enc_form_f32(uint32_t d, int form);
+// fp32 tensors and matrix products (k_attn_enc_f32.hip), or fp16.
+void launch_attn_enc_f16(const AttnEncArgs& a, uint32_t B, int form, hipStream_t s);
+void launch_attn_enc_f32(const AttnEncArgs& a, uint32_t B, int form, hipStream_t s);
 
 }  // namespace di

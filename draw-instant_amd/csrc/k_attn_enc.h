@@ -25,15 +25,19 @@
 // with a zero sum and store zeros.
 //
 // Keys come in tiles of KT through LDS (loads go straight to LDS; 16-byte
-// chunks XOR-swizzled by row so that fragment reads meet no bank twice), two
-// buffers, the next tile in flight while one is computed.  Rows are padded to
-// DK channels in registers and to a power of two of chunks in LDS; chunks past
-// d and keys past the length are never read from memory and land as zeros.
+// chunks XOR-swizzled by row so that fragment reads meet no bank twice).  Rows
+// are padded to DK channels in registers and to a power of two of chunks in LDS;
+// chunks past d and keys past the length are never read from memory and land
+// as zeros.  The loop is pipelined over tiles: the scores of tile t + 1 are
+// multiplied between the exponentials of tile t, so that a wavefront has
+// matrix and vector work at once, then tile t's probabilities meet its values.
+// K is therefore fetched two tiles ahead and V one, each into two buffers.
 //
 // WM wavefronts share a tile, each with QG groups of 16 rows; WK such groups
 // of wavefronts walk different tiles of the same rows and are merged through
-// LDS.  Many rows: WM = 4, WK = 1.  Few rows (a token, a handful of
-// latents): WM = 1, WK = 4, so that every wavefront streams keys of its own.
+// LDS.  Forms: many rows, WM = 4 and QG = 2 (two groups share every fragment
+// read); up to 64 rows, WM = 4 and QG = 1; few rows (a token, a handful of
+// latents), WM = 1 and WK = 4, so that every wavefront streams keys of its own.
 // Where the rows still leave CUs idle the keys are split over workgroups as
 // well and k_attn_enc_merge joins the parts.
 #pragma once
@@ -60,7 +64,10 @@ constexpr float kLowest = -3.0e38f;        // the lowest one in log2 units: abov
 // so none exceeds it either (fp16 max is 65504)
 constexpr uint32_t kLaneSumMaxBits = 0x47000000u;  // 32768.0f
 constexpr float kLog2E = 1.4426950408889634f;
-constexpr int kWaitAll = (7 << 4);  // s_waitcnt vmcnt(0) lgkmcnt(0), expcnt not waited on
+// s_waitcnt: all but the last n vector memory operations; the same and all LDS
+// operations
+constexpr int wait_vm(int n) { return (n & 15) | (n >> 4) << 14 | 7 << 4 | 15 << 8; }
+constexpr int wait_vm_lds(int n) { return (n & 15) | (n >> 4) << 14 | 7 << 4; }
 
 template <int N>
 using Int = std::integral_constant<int, N>;
@@ -90,9 +97,10 @@ __device__ __forceinline__ float enc_sum4(float x) {
 }
 
 // Shapes of one instantiation.
-template <typename T, int DK, bool FEW>
+template <typename T, int DK, int FORM>
 struct EncShape {
   static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr bool FEW = FORM == ENC_FEW;
   static constexpr int EPC = 16 / sizeof(T);  // elements per 16-byte chunk
   // chunks of an LDS row: a power of two
   static constexpr int C0 = DK / EPC;
@@ -104,18 +112,20 @@ struct EncShape {
   static constexpr int WM = FEW ? 1 : 4;
   // four wavefronts' buffers while they fit the 160 KiB of LDS
   static constexpr int WK = FEW ? (TILE * 4 * 4 <= 128 * 1024 ? 4 : 2) : 1;
-  static constexpr int QG = FEW || F32 || DK > 128 ? 1 : 2;
+  // two row groups where their accumulators leave room for two wavefronts a SIMD
+  static constexpr int QG = FORM == ENC_MANY && !F32 && DK <= 128 ? 2 : 1;
   static constexpr int ROWS = WM * QG * 16;
   static constexpr int NT = WM * WK * 64;
-  static constexpr int LDS = WK * 4 * TILE;  // [key group][buffer][K | V]
+  static constexpr int LDS = WK * 4 * TILE;  // [key group][K | V][buffer]
   // wavefronts per SIMD that registers are kept for: what the LDS lets reside
-  static constexpr int WAVES = LDS * 2 <= 160 * 1024 ? 2 : 1;
+  // (fp32 at 256 channels takes more than half of a SIMD's registers)
+  static constexpr int WAVES = LDS * 2 <= 160 * 1024 && !(F32 && DK > 192) ? 2 : 1;
 };
 
-template <typename T, int DK, bool FEW, bool BIAS>
-__global__ __launch_bounds__((EncShape<T, DK, FEW>::NT), (EncShape<T, DK, FEW>::WAVES))
+template <typename T, int DK, int FORM, bool BIAS>
+__global__ __launch_bounds__((EncShape<T, DK, FORM>::NT), (EncShape<T, DK, FORM>::WAVES))
 void k_attn_enc(AttnEncArgs a) {
-  typedef EncShape<T, DK, FEW> Sh;
+  typedef EncShape<T, DK, FORM> Sh;
   constexpr bool F32 = Sh::F32;
   constexpr int EPC = Sh::EPC, CPR = Sh::CPR, KT = Sh::KT, TILE = Sh::TILE, WM = Sh::WM, WK = Sh::WK;
   constexpr int QG = Sh::QG, NKT = KT / 16, NDT = DK / 16;
@@ -213,19 +223,22 @@ void k_attn_enc(AttnEncArgs a) {
     dk[i] = ck * EPC < a.d ? kr * (uint32_t)(a.ldk * sizeof(T)) + ck * 16u : 0x80000000u;
     dv[i] = cv * EPC < a.d ? kr * (uint32_t)(a.ldv * sizeof(T)) + cv * 16u : 0x80000000u;
   }
-  auto fetch = [&](int t, auto buf_c) {
+  unsigned char* const lds = smem + kg * 4 * TILE;
+  auto fetch_k = [&](int t, auto buf_c) {
     const uint32_t key0 = (uint32_t)t * KT, left = min(nk - key0, (uint32_t)KT);
-    const __amdgpu_buffer_rsrc_t rK = enc_rsrc(K + (uint64_t)key0 * a.ldk,
+    const __amdgpu_buffer_rsrc_t rs = enc_rsrc(K + (uint64_t)key0 * a.ldk,
                                                (uint32_t)(((left - 1) * a.ldk + a.d) * sizeof(T)));
-    const __amdgpu_buffer_rsrc_t rV = enc_rsrc(V + (uint64_t)key0 * a.ldv,
+    unsigned char* base = lds + decltype(buf_c)::value * TILE + wm * NI * 1024;
+#pragma unroll
+    for (int i = 0; i < NI; i++) load_lds16(rs, base + i * 1024, dk[i]);
+  };
+  auto fetch_v = [&](int t, auto buf_c) {
+    const uint32_t key0 = (uint32_t)t * KT, left = min(nk - key0, (uint32_t)KT);
+    const __amdgpu_buffer_rsrc_t rs = enc_rsrc(V + (uint64_t)key0 * a.ldv,
                                                (uint32_t)(((left - 1) * a.ldv + a.d) * sizeof(T)));
-    unsigned char* base = smem + (kg * 2 + decltype(buf_c)::value) * 2 * TILE + wm * NI * 1024;
+    unsigned char* base = lds + (2 + decltype(buf_c)::value) * TILE + wm * NI * 1024;
 #pragma unroll
-    for (int i = 0; i < NI; i++)
-      load_lds16(rK, base + i * 1024, dk[i]);
-#pragma unroll
-    for (int i = 0; i < NI; i++)
-      load_lds16(rV, base + TILE + i * 1024, dv[i]);
+    for (int i = 0; i < NI; i++) load_lds16(rs, base + i * 1024, dv[i]);
   };
 
   // K fragment c of 16-key tile kt: row kt * 16 + r, chunk 4 c + g
@@ -238,9 +251,9 @@ void k_attn_enc(AttnEncArgs a) {
 #pragma unroll
   for (int dt = 0; dt < NDT; dt++) {
     if constexpr (F32)
-      v_rd[dt] = TILE + 4 * g * RB + (((4 * dt + (r >> 2)) ^ vswz(4 * g)) << 4) + (r & 3) * 4;
+      v_rd[dt] = 2 * TILE + 4 * g * RB + (((4 * dt + (r >> 2)) ^ vswz(4 * g)) << 4) + (r & 3) * 4;
     else
-      v_rd[dt] = TILE + (4 * g + (r >> 2)) * RB +
+      v_rd[dt] = 2 * TILE + (4 * g + (r >> 2)) * RB +
                  (((2 * dt + ((r & 3) >> 1)) ^ vswz(4 * g + (r >> 2))) << 4) + (r & 1) * 8;
   }
 
@@ -254,203 +267,239 @@ void k_attn_enc(AttnEncArgs a) {
     for (int dt = 0; dt < NDT; dt++) o[i][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  auto tile = [&](auto cur_c, int t) {
-    constexpr int cur = decltype(cur_c)::value;
-    const unsigned char* sb = smem + (kg * 2 + cur) * 2 * TILE;
-    if (t < t1) {
-      if (t + 1 < t1) fetch(t + 1, Int<cur ^ 1>{});
-      const uint32_t key0 = (uint32_t)t * KT;
-      const bool ragged = key0 + KT > nk;
-      f32x4 bb[BIAS ? QG : 1][BIAS ? NKT : 1];
-      if constexpr (BIAS) {
-        // in flight while the scores are computed; past the last key: unread
+  // q k^T of tile t, in K buffer `buf`; keys past the last are -inf
+  auto scores = [&](int t, auto buf_c, f32x4 (&s)[QG][NKT]) {
+    const unsigned char* sb = lds + decltype(buf_c)::value * TILE;
 #pragma unroll
-        for (int i = 0; i < QG; i++)
+    for (int kt = 0; kt < NKT; kt++) {
 #pragma unroll
-          for (int kt = 0; kt < NKT; kt++) {
-            const uint32_t key = key0 + kt * 16 + 4 * g;
-            if (!ragged) {
-              bb[i][kt] = *(const f32x4u*)(bp[i] + key);
-            } else {
+      for (int i = 0; i < QG; i++) s[i][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-              for (int j = 0; j < 4; j++) bb[i][kt][j] = key + j < nk ? bp[i][key + j] : -INFINITY;
-            }
-          }
-      }
-      f32x4 s[QG][NKT];
+      for (int c = 0; c < QC; c++) {
+        const frag kf = *(const frag*)(sb + k_rd[c] + kt * 16 * RB);
 #pragma unroll
-      for (int kt = 0; kt < NKT; kt++) {
+        for (int i = 0; i < QG; i++) {
+          if constexpr (F32) {
 #pragma unroll
-        for (int i = 0; i < QG; i++) s[i][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < QC; c++) {
-          const frag kf = *(const frag*)(sb + k_rd[c] + kt * 16 * RB);
-#pragma unroll
-          for (int i = 0; i < QG; i++) {
-            if constexpr (F32) {
-#pragma unroll
-              for (int j = 0; j < 4; j++)
-                s[i][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qf[i][c][j], s[i][kt], 0, 0, 0);
-            } else {
-              s[i][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[i][c], s[i][kt], 0, 0, 0);
-            }
+            for (int j = 0; j < 4; j++)
+              s[i][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qf[i][c][j], s[i][kt], 0, 0, 0);
+          } else {
+            s[i][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[i][c], s[i][kt], 0, 0, 0);
           }
         }
       }
-      if (ragged) {
+    }
+  };
+  auto cut = [&](int t, f32x4 (&s)[QG][NKT]) {
+    const uint32_t key0 = (uint32_t)t * KT;
+    if (key0 + KT <= nk) return;
 #pragma unroll
-        for (int kt = 0; kt < NKT; kt++)
+    for (int kt = 0; kt < NKT; kt++)
 #pragma unroll
-          for (int j = 0; j < 4; j++)
-            if (key0 + kt * 16 + 4 * g + j >= nk) {
+      for (int j = 0; j < 4; j++)
+        if (key0 + kt * 16 + 4 * g + j >= nk) {
 #pragma unroll
-              for (int i = 0; i < QG; i++) s[i][kt][j] = -INFINITY;
-            }
-      }
-      bool removed = false;  // some query of this wavefront does not see some key
-      if constexpr (BIAS) {
+          for (int i = 0; i < QG; i++) s[i][kt][j] = -INFINITY;
+        }
+  };
+  // the bias of tile t on its way (past the last key: unread), and the current one
+  f32x4 bb[BIAS ? QG : 1][BIAS ? NKT : 1], bn[BIAS ? QG : 1][BIAS ? NKT : 1];
+  auto load_bias = [&](int t) {
+    if constexpr (BIAS) {
+      const uint32_t key0 = (uint32_t)t * KT;
 #pragma unroll
-        for (int i = 0; i < QG; i++)
+      for (int i = 0; i < QG; i++)
 #pragma unroll
-          for (int kt = 0; kt < NKT; kt++)
+        for (int kt = 0; kt < NKT; kt++) {
+          const uint32_t key = key0 + kt * 16 + 4 * g;
+          if (key0 + KT <= nk) {
+            bn[i][kt] = *(const f32x4u*)(bp[i] + key);
+          } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-              const float x = bb[i][kt][j];
-              removed |= x == -INFINITY;
-              if (x <= kSwamped) s[i][kt][j] = 0.0f;  // whatever the score: it may be NaN
-              // in log2 units; the product of a finite bias stays finite
-              bb[i][kt][j] = x == -INFINITY ? x : fmaxf(x * kLog2E, kLowest);
-            }
-      }
-      // in log2 units
-      auto score = [&](int i, int kt, int j) -> float {
-        if constexpr (BIAS) return fmaf(s[i][kt][j], a.scale_log2, bb[i][kt][j]);
-        else return s[i][kt][j] * a.scale_log2;
-      };
-      // raise the running maximum to this tile's where that is larger
-      auto raise = [&](int i) {
-        float mx = score(i, 0, 0);
+            for (int j = 0; j < 4; j++) bn[i][kt][j] = key + j < nk ? bp[i][key + j] : -INFINITY;
+          }
+        }
+    }
+  };
+  // the loaded bias in log2 units and its effect on scores that do not count;
+  // whether some row of this wavefront does not see some key
+  auto apply_bias = [&](f32x4 (&s)[QG][NKT]) -> bool {
+    bool removed = false;
+    if constexpr (BIAS) {
 #pragma unroll
-        for (int kt = 0; kt < NKT; kt++)
-#pragma unroll
-          for (int j = 0; j < 4; j++) mx = fmaxf(mx, score(i, kt, j));
-        mx = fmaxf(enc_max4(mx), m[i]);
-        const float al = m[i] == kNone ? 0.0f : __builtin_amdgcn_exp2f(m[i] - mx);
-        m[i] = mx;
-        l[i] *= al;
-#pragma unroll
-        for (int dt = 0; dt < NDT; dt++) o[i][dt] *= al;
-      };
-      float pr[QG][NKT][4], ts[QG];
-      auto probs = [&](int i) {
-        ts[i] = 0.0f;
+      for (int i = 0; i < QG; i++)
 #pragma unroll
         for (int kt = 0; kt < NKT; kt++)
 #pragma unroll
           for (int j = 0; j < 4; j++) {
-            // with a bias, (bias - m) first: it is exact where they are close
-            const float x = fmaf(s[i][kt][j], a.scale_log2, BIAS ? bb[i][kt][j] - m[i] : -m[i]);
-            pr[i][kt][j] = __builtin_amdgcn_exp2f(x);
-            ts[i] += pr[i][kt][j];
+            const float x = bn[i][kt][j];
+            removed |= x == -INFINITY;
+            if (x <= kSwamped) s[i][kt][j] = 0.0f;  // whatever the score: it may be NaN
+            // (the product of a finite bias stays finite)
+            bb[i][kt][j] = x == -INFINITY ? x : fmaxf(x * kLog2E, kLowest);
           }
-      };
+    }
+    return __builtin_amdgcn_ballot_w64(removed) != 0;
+  };
+  // raise the running maximum to this tile's where that is larger
+  auto raise = [&](int i, f32x4 (&s)[QG][NKT]) {
+    float mx = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < QG; i++) {
-        // rows without a key so far: take the maximum
-        if (__builtin_amdgcn_ballot_w64(m[i] == kNone) != 0) raise(i);
-        probs(i);
-        // a probability above 2^15 (or inf / NaN) shows in its lane's sum; the
-        // bits' order puts finite < inf < NaN
-        if (__builtin_amdgcn_ballot_w64((__float_as_uint(ts[i]) & 0x7fffffffu) > kLaneSumMaxBits) != 0) {
-          raise(i);
-          probs(i);
-        }
-        l[i] += ts[i];
+    for (int kt = 0; kt < NKT; kt++)
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        mx = fmaxf(mx, BIAS ? fmaf(s[i][kt][j], a.scale_log2, bb[i][kt][j]) : s[i][kt][j]);
+    mx = fmaxf(BIAS ? enc_max4(mx) : enc_max4(mx) * a.scale_log2, m[i]);
+    const float al = m[i] == kNone ? 0.0f : __builtin_amdgcn_exp2f(m[i] - mx);
+    m[i] = mx;
+    l[i] *= al;
+#pragma unroll
+    for (int dt = 0; dt < NDT; dt++) o[i][dt] *= al;
+  };
+  // probabilities, and their sum over this lane's keys.  A row without a key
+  // so far has m = kNone: its first ones come out infinite.
+  float pr[QG][NKT][4], ts[QG];
+  auto probs = [&](int i, f32x4 (&s)[QG][NKT]) {
+    ts[i] = 0.0f;
+#pragma unroll
+    for (int kt = 0; kt < NKT; kt++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        // with a bias, (bias - m) first: it is exact where they are close
+        pr[i][kt][j] = __builtin_amdgcn_exp2f(fmaf(s[i][kt][j], a.scale_log2, BIAS ? bb[i][kt][j] - m[i] : -m[i]));
+        ts[i] += pr[i][kt][j];
       }
-      // O^T += V^T P^T.  MASKED: the values of keys that none of this
-      // wavefront's rows sees become zeros (0 * NaN would not vanish).
-      uint32_t seen = ~0u;  // bit 4 kt + j: key kt * 16 + 4g + j
-      if constexpr (BIAS) {
-        if (__builtin_amdgcn_ballot_w64(removed) != 0) {
-          seen = 0;
+  };
+  // O^T += V^T P^T with tile t's values, in V buffer `buf`.  MASKED: the values
+  // of keys that none of this wavefront's rows sees (`seen` bit 4 kt + j: key kt *
+  // 16 + 4g + j) become zeros, as 0 * NaN would not vanish.
+  auto values = [&](auto buf_c, auto masked_c, uint32_t seen) {
+    constexpr bool MASKED = decltype(masked_c)::value != 0;
+    const unsigned char* sb = lds + decltype(buf_c)::value * TILE;
+    if constexpr (F32) {
 #pragma unroll
-          for (int kt = 0; kt < NKT; kt++)
+      for (int kt = 0; kt < NKT; kt++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-              bool some = false;
+        for (int j = 0; j < 4; j++)
 #pragma unroll
-              for (int i = 0; i < QG; i++) some |= live[i] && bb[i][kt][j] > -INFINITY;
-              const uint64_t bal = __builtin_amdgcn_ballot_w64(some);
-              seen |= (((bal >> (16 * g)) & 0xffffu) != 0 ? 1u : 0u) << (4 * kt + j);
-            }
-        }
-      }
-      auto pv = [&](auto masked_c) {
-        constexpr bool MASKED = decltype(masked_c)::value != 0;
-        if constexpr (F32) {
-#pragma unroll
-          for (int kt = 0; kt < NKT; kt++)
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-#pragma unroll
-              for (int dt = 0; dt < NDT; dt++) {
-                float vf = *(const float*)(sb + v_rd[dt] + (kt * 16 + j) * RB);
-                if constexpr (MASKED) vf = (seen >> (4 * kt + j)) & 1u ? vf : 0.0f;
-#pragma unroll
-                for (int i = 0; i < QG; i++)
-                  o[i][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf, pr[i][kt][j], o[i][dt], 0, 0, 0);
-              }
-        } else {
-#pragma unroll
-          for (int c = 0; c < NKT / 2; c++) {
-            f16x8 pf[QG];
+          for (int dt = 0; dt < NDT; dt++) {
+            float vf = *(const float*)(sb + v_rd[dt] + (kt * 16 + j) * RB);
+            if constexpr (MASKED) vf = (seen >> (4 * kt + j)) & 1u ? vf : 0.0f;
 #pragma unroll
             for (int i = 0; i < QG; i++)
-#pragma unroll
-              for (int j = 0; j < 8; j++) pf[i][j] = (f16)pr[i][2 * c + j / 4][j % 4];
-            u32x4 keep = {~0u, ~0u, ~0u, ~0u};
-            if constexpr (MASKED) {
-#pragma unroll
-              for (int j = 0; j < 4; j++)
-                keep[j] = ((seen >> (8 * c + 2 * j)) & 1u ? 0xffffu : 0u) |
-                          ((seen >> (8 * c + 2 * j + 1)) & 1u ? 0xffff0000u : 0u);
-            }
-#pragma unroll
-            for (int dt = 0; dt < NDT; dt++) {
-              const unsigned char* vp = sb + v_rd[dt] + c * 32 * RB;
-              const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)vp);
-              const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vp + 16 * RB));
-              f16x8 vf = __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-              if constexpr (MASKED)
-                vf = __builtin_bit_cast(f16x8, __builtin_bit_cast(u32x4, vf) & keep);
-#pragma unroll
-              for (int i = 0; i < QG; i++)
-                o[i][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[i], o[i][dt], 0, 0, 0);
-            }
+              o[i][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf, pr[i][kt][j], o[i][dt], 0, 0, 0);
           }
+    } else {
+#pragma unroll
+      for (int c = 0; c < NKT / 2; c++) {
+        f16x8 pf[QG];
+#pragma unroll
+        for (int i = 0; i < QG; i++)
+#pragma unroll
+          for (int j = 0; j < 8; j++) pf[i][j] = (f16)pr[i][2 * c + j / 4][j % 4];
+        u32x4 keep = {~0u, ~0u, ~0u, ~0u};
+        if constexpr (MASKED) {
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            keep[j] = ((seen >> (8 * c + 2 * j)) & 1u ? 0xffffu : 0u) |
+                      ((seen >> (8 * c + 2 * j + 1)) & 1u ? 0xffff0000u : 0u);
         }
-      };
-      if (BIAS && __builtin_amdgcn_ballot_w64(removed) != 0) pv(Int<1>{});
-      else pv(Int<0>{});
+#pragma unroll
+        for (int dt = 0; dt < NDT; dt++) {
+          const unsigned char* vp = sb + v_rd[dt] + c * 32 * RB;
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)vp);
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vp + 16 * RB));
+          f16x8 vf = __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+          if constexpr (MASKED) vf = __builtin_bit_cast(f16x8, __builtin_bit_cast(u32x4, vf) & keep);
+#pragma unroll
+          for (int i = 0; i < QG; i++)
+            o[i][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[i], o[i][dt], 0, 0, 0);
+        }
+      }
     }
-    // the next tile has landed, and every wavefront that shares it is done with
-    // this one (a wavefront with tiles of its own waits for itself alone)
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-    __builtin_amdgcn_s_waitcnt(kWaitAll);
+  };
+  // Every load but the last n of this wavefront's has landed, and its LDS reads
+  // are done; wavefronts that share tiles meet.
+  auto meet = [&](auto n_c) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_waitcnt(wait_vm_lds(decltype(n_c)::value));
     if constexpr (WM > 1) __builtin_amdgcn_s_barrier();
     else __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
   };
 
-  if (t0 < t1) fetch(t0, Int<0>{});
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-  __builtin_amdgcn_s_waitcnt(kWaitAll);
-  __syncthreads();
-  // two tiles per iteration so that each LDS buffer has fixed offsets; every
-  // wavefront of the workgroup makes tpg iterations
-  for (int i = 0; i < tpg; i += 2) {
-    tile(Int<0>{}, t0 + i);
-    if (i + 1 < tpg) tile(Int<1>{}, t0 + i + 1);
+  // Tile t with its scores in `s`; those of t + 1 go to `sn`.
+  auto step = [&](auto cur_c, int t, f32x4 (&s)[QG][NKT], f32x4 (&sn)[QG][NKT]) {
+    constexpr int cur = decltype(cur_c)::value;
+    if (t + 2 < t1) fetch_k(t + 2, Int<cur>{});
+    if (t + 1 < t1) fetch_v(t + 1, Int<cur ^ 1>{});
+    const bool removed = apply_bias(s);
+    if (t + 1 < t1) {
+      load_bias(t + 1);
+      scores(t + 1, Int<cur ^ 1>{}, sn);
+#pragma unroll
+      for (int i = 0; i < QG; i++) probs(i, s);
+    } else {
+#pragma unroll
+      for (int i = 0; i < QG; i++) probs(i, s);
+    }
+#pragma unroll
+    for (int i = 0; i < QG; i++) {
+      // a probability above 2^15 (or inf / NaN) shows in its lane's sum; the
+      // bits' order puts finite < inf < NaN
+      if (__builtin_amdgcn_ballot_w64((__float_as_uint(ts[i]) & 0x7fffffffu) > kLaneSumMaxBits) != 0) {
+        raise(i, s);
+        probs(i, s);
+      }
+      l[i] += ts[i];
+    }
+    if (BIAS && removed) {
+      uint32_t seen = 0;
+#pragma unroll
+      for (int kt = 0; kt < NKT; kt++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          bool some = false;
+#pragma unroll
+          for (int i = 0; i < QG; i++) some |= live[i] && bb[BIAS ? i : 0][BIAS ? kt : 0][j] > -INFINITY;
+          const uint64_t bal = __builtin_amdgcn_ballot_w64(some);
+          seen |= (((bal >> (16 * g)) & 0xffffu) != 0 ? 1u : 0u) << (4 * kt + j);
+        }
+      values(cur_c, Int<1>{}, seen);
+    } else {
+      values(cur_c, Int<0>{}, 0u);
+    }
+    if (t + 1 < t1) {
+      cut(t + 1, sn);
+      meet(Int<0>{});
+    }
+  };
+
+  if (t0 < t1) {
+    fetch_k(t0, Int<0>{});
+    fetch_v(t0, Int<0>{});
+    if (t0 + 1 < t1) {
+      fetch_k(t0 + 1, Int<1>{});
+      meet(Int<2 * NI>{});
+    } else {
+      meet(Int<NI>{});
+    }
+    f32x4 s0[QG][NKT], s1[QG][NKT];
+    load_bias(t0);
+    scores(t0, Int<0>{}, s0);
+    cut(t0, s0);
+    meet(Int<0>{});
+    bool first = true;
+    // two tiles per iteration so that each LDS buffer has fixed offsets
+    for (int t = t0; t < t1; t += 2) {
+      if (!BIAS && first) {
+#pragma unroll
+        for (int i = 0; i < QG; i++) raise(i, s0);
+        first = false;
+      }
+      step(Int<0>{}, t, s0, s1);
+      if (t + 1 < t1) step(Int<1>{}, t + 1, s1, s0);
+    }
   }
 #pragma unroll
   for (int i = 0; i < QG; i++) l[i] = enc_sum4(l[i]);
@@ -460,7 +509,7 @@ void k_attn_enc(AttnEncArgs a) {
     // l at [f][l]; group 0 rescales every part to the largest maximum
     static_assert(WK == 1 || QG == 1, "key groups with one row group");
     constexpr int NF = NDT * 4 + 2;
-    static_assert((WK - 1) * WM * NF * 64 * 4 <= (int)sizeof(smem), "the parts fit the buffers");
+    static_assert((WK - 1) * WM * NF * 64 * 4 <= Sh::LDS, "the parts fit the buffers");
     float* xs = reinterpret_cast<float*>(smem);
     __syncthreads();  // the buffers are free
     if (kg > 0) {
@@ -519,99 +568,144 @@ void k_attn_enc(AttnEncArgs a) {
   }
 }
 
-// Joins the key ranges: one thread per 4 channels of a row, the ranges in order.
+// Joins the key ranges.  A workgroup of 256 threads takes rows of d / 4 vectors:
+// SG threads per vector, thread g of them the ranges g, g + SG, .. in order,
+// then their partial sums through LDS in order of g.
 template <typename T>
-__global__ __launch_bounds__(256) void k_attn_enc_merge(AttnEncArgs a) {
+__global__ __launch_bounds__(256) void k_attn_enc_merge(AttnEncArgs a, uint32_t SG) {
+  __shared__ float sm[256 * 6];
   kernarg_warm(a);
-  const uint32_t vpr = a.d / 4;
-  const uint64_t total = a.prows * vpr, step = (uint64_t)gridDim.x * 256;
-  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
-    const uint64_t row = i / vpr;
-    const uint32_t c = (uint32_t)(i - row * vpr) * 4;
-    float mx = kNone, l = 0.0f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t s0 = 0; s0 < a.splits; s0 += 4) {
-      float2 ml[4];
-      f32x4 v[4];
+  const uint32_t vpr = a.d / 4, per = 256 / SG;  // vectors per workgroup
+  const uint32_t sg = threadIdx.x / per, vi = threadIdx.x % per;
+  const uint64_t i = (uint64_t)blockIdx.x * per + vi, total = a.prows * vpr;
+  const bool ok = i < total && sg < SG;
+  const uint64_t row = ok ? i / vpr : 0;
+  const uint32_t c = ok ? (uint32_t)(i - row * vpr) * 4 : 0;
+  float mx = kNone, l = 0.0f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (uint32_t s0 = sg; ok && s0 < a.splits; s0 += SG * 4) {
+    float2 ml[4];
+    f32x4 v[4];
 #pragma unroll
-      for (uint32_t u = 0; u < 4; u++) {
-        const uint64_t p = (uint64_t)min(s0 + u, a.splits - 1) * a.prows + row;
-        ml[u] = *(const float2*)(a.part_ml + p * 2);
-        v[u] = *(const f32x4*)(a.part_o + p * a.d + c);
-      }
-      float m2 = mx;
-#pragma unroll
-      for (uint32_t u = 0; u < 4; u++) m2 = fmaxf(m2, ml[u].x);
-      const float al = __builtin_amdgcn_exp2f(mx - m2);
-      l *= al;
-      acc *= al;
-      mx = m2;
-#pragma unroll
-      for (uint32_t u = 0; u < 4; u++) {
-        if (s0 + u >= a.splits || ml[u].y == 0.0f) continue;  // (an empty range adds nothing)
-        const float wt = __builtin_amdgcn_exp2f(ml[u].x - mx);
-        l += wt * ml[u].y;
-        acc += wt * v[u];
-      }
+    for (uint32_t u = 0; u < 4; u++) {
+      const uint64_t p = (uint64_t)min(s0 + u * SG, a.splits - 1) * a.prows + row;
+      ml[u] = *(const float2*)(a.part_ml + p * 2);
+      v[u] = *(const f32x4*)(a.part_o + p * a.d + c);
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const uint32_t rr = (uint32_t)(row % a.rows), q = rr / a.G;
-    const uint64_t hb = row / a.rows;
-    const uint64_t h = (hb % a.Hk) * a.G + (rr - q * a.G), b = hb / a.Hk;
-    T* dst = (T*)a.o + b * a.bo + h * a.ho + (uint64_t)q * a.ldo + c;
-    const f32x4 v = acc * inv;
-    if constexpr (sizeof(T) == 4) *(f32x4*)dst = v;
-    else *(f16x4*)dst = f16x4{(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3]};
+    float m2 = mx;
+#pragma unroll
+    for (uint32_t u = 0; u < 4; u++) m2 = fmaxf(m2, ml[u].x);
+    const float al = __builtin_amdgcn_exp2f(mx - m2);
+    l *= al;
+    acc *= al;
+    mx = m2;
+#pragma unroll
+    for (uint32_t u = 0; u < 4; u++) {
+      if (s0 + u * SG >= a.splits || ml[u].y == 0.0f) continue;  // (an empty range adds nothing)
+      const float wt = __builtin_amdgcn_exp2f(ml[u].x - mx);
+      l += wt * ml[u].y;
+      acc += wt * v[u];
+    }
   }
+  float* own = sm + threadIdx.x * 6;
+  own[0] = mx;
+  own[1] = l;
+#pragma unroll
+  for (int j = 0; j < 4; j++) own[2 + j] = acc[j];
+  __syncthreads();
+  if (!ok || sg > 0) return;
+  float m2 = mx;
+  for (uint32_t k = 1; k < SG; k++) m2 = fmaxf(m2, sm[(k * per + vi) * 6]);
+  float wt = __builtin_amdgcn_exp2f(mx - m2);
+  l *= wt;
+  acc *= wt;
+  for (uint32_t k = 1; k < SG; k++) {
+    const float* o = sm + (k * per + vi) * 6;
+    if (o[1] == 0.0f) continue;
+    wt = __builtin_amdgcn_exp2f(o[0] - m2);
+    l += wt * o[1];
+#pragma unroll
+    for (int j = 0; j < 4; j++) acc[j] += wt * o[2 + j];
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const uint32_t rr = (uint32_t)(row % a.rows), q = rr / a.G;
+  const uint64_t hb = row / a.rows;
+  const uint64_t h = (hb % a.Hk) * a.G + (rr - q * a.G), b = hb / a.Hk;
+  T* dst = (T*)a.o + b * a.bo + h * a.ho + (uint64_t)q * a.ldo + c;
+  const f32x4 v = acc * inv;
+  if constexpr (sizeof(T) == 4) *(f32x4*)dst = v;
+  else *(f16x4*)dst = f16x4{(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3]};
 }
 
-template <typename T, int DK, bool FEW>
+template <typename T, int DK, int FORM>
 void launch_enc_form(const AttnEncArgs& a, uint32_t B, hipStream_t s) {
+  typedef EncShape<T, DK, FORM> Sh;
   const dim3 grid(a.blocks * a.splits * a.Hk * B);
-  if (a.bias) k_attn_enc<T, DK, FEW, true><<<grid, EncShape<T, DK, FEW>::NT, 0, s>>>(a);
-  else k_attn_enc<T, DK, FEW, false><<<grid, EncShape<T, DK, FEW>::NT, 0, s>>>(a);
+  if constexpr (enc_bias_ok(DK, FORM))
+    if (a.bias) {
+      k_attn_enc<T, DK, FORM, true><<<grid, Sh::NT, 0, s>>>(a);
+      return;
+    }
+  k_attn_enc<T, DK, FORM, false><<<grid, Sh::NT, 0, s>>>(a);
 }
 
 template <typename T, int DK>
-void launch_enc_dk(const AttnEncArgs& a, uint32_t B, bool few, hipStream_t s) {
-  if (few) launch_enc_form<T, DK, true>(a, B, s);
-  else launch_enc_form<T, DK, false>(a, B, s);
+void launch_enc_dk(const AttnEncArgs& a, uint32_t B, int form, hipStream_t s) {
+  if (form == ENC_FEW) {
+    launch_enc_form<T, DK, ENC_FEW>(a, B, s);
+    return;
+  }
+  // (one row group a wavefront in either form: one kernel)
+  if constexpr (EncShape<T, DK, ENC_MANY>::QG > 1) {
+    if (form == ENC_MANY) {
+      launch_enc_form<T, DK, ENC_MANY>(a, B, s);
+      return;
+    }
+  }
+  launch_enc_form<T, DK, ENC_MID>(a, B, s);
 }
 
 // d padded to the channels of an instantiation
 inline uint32_t enc_channels(uint32_t d) { return d <= 192 ? (d + 31) / 32 * 32 : 256; }
 
-template <typename T, bool FEW>
-AttnEncForm enc_form(uint32_t d) {
+template <typename T, int DK>
+AttnEncForm enc_form_dk(int form) {
   auto of = [](auto s) {
     typedef decltype(s) S;
     return AttnEncForm{S::ROWS, S::KT, S::WK};
   };
+  return form == ENC_FEW ? of(EncShape<T, DK, ENC_FEW>{})
+                         : form == ENC_MID ? of(EncShape<T, DK, ENC_MID>{}) : of(EncShape<T, DK, ENC_MANY>{});
+}
+
+template <typename T>
+AttnEncForm enc_form(uint32_t d, int form) {
   switch (enc_channels(d)) {
-    case 32: return of(EncShape<T, 32, FEW>{});
-    case 64: return of(EncShape<T, 64, FEW>{});
-    case 96: return of(EncShape<T, 96, FEW>{});
-    case 128: return of(EncShape<T, 128, FEW>{});
-    case 160: return of(EncShape<T, 160, FEW>{});
-    case 192: return of(EncShape<T, 192, FEW>{});
-    default: return of(EncShape<T, 256, FEW>{});
+    case 32: return enc_form_dk<T, 32>(form);
+    case 64: return enc_form_dk<T, 64>(form);
+    case 96: return enc_form_dk<T, 96>(form);
+    case 128: return enc_form_dk<T, 128>(form);
+    case 160: return enc_form_dk<T, 160>(form);
+    case 192: return enc_form_dk<T, 192>(form);
+    default: return enc_form_dk<T, 256>(form);
   }
 }
 
 template <typename T>
-void launch_enc(const AttnEncArgs& a, uint32_t B, bool few, hipStream_t s) {
+void launch_enc(const AttnEncArgs& a, uint32_t B, int form, hipStream_t s) {
   switch (enc_channels(a.d)) {
-    case 32: launch_enc_dk<T, 32>(a, B, few, s); break;
-    case 64: launch_enc_dk<T, 64>(a, B, few, s); break;
-    case 96: launch_enc_dk<T, 96>(a, B, few, s); break;
-    case 128: launch_enc_dk<T, 128>(a, B, few, s); break;
-    case 160: launch_enc_dk<T, 160>(a, B, few, s); break;
-    case 192: launch_enc_dk<T, 192>(a, B, few, s); break;
-    default: launch_enc_dk<T, 256>(a, B, few, s); break;
+    case 32: launch_enc_dk<T, 32>(a, B, form, s); break;
+    case 64: launch_enc_dk<T, 64>(a, B, form, s); break;
+    case 96: launch_enc_dk<T, 96>(a, B, form, s); break;
+    case 128: launch_enc_dk<T, 128>(a, B, form, s); break;
+    case 160: launch_enc_dk<T, 160>(a, B, form, s); break;
+    case 192: launch_enc_dk<T, 192>(a, B, form, s); break;
+    default: launch_enc_dk<T, 256>(a, B, form, s); break;
   }
   if (a.splits > 1) {
-    const uint64_t blocks = (a.prows * (a.d / 4) + 255) / 256;
-    k_attn_enc_merge<T><<<(uint32_t)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(a);
+    // threads per vector: four ranges each
+    const uint32_t sg = a.splits <= 4 ? 1 : a.splits <= 8 ? 2 : a.splits <= 16 ? 4 : 8, per = 256 / sg;
+    k_attn_enc_merge<T><<<(uint32_t)((a.prows * (a.d / 4) + per - 1) / per), 256, 0, s>>>(a, sg);
   }
 }
 

@@ -7,13 +7,11 @@
 
 namespace di {
 
-void launch_attn_enc_f16(const AttnEncArgs& a, uint32_t B, bool few, hipStream_t s) {
-  launch_enc<f16>(a, B, few, s);
+void launch_attn_enc_f16(const AttnEncArgs& a, uint32_t B, int form, hipStream_t s) {
+  launch_enc<f16>(a, B, form, s);
 }
 
-AttnEncForm attn_enc_form_f16(uint32_t d, bool few) {
-  return few ? enc_form<f16, true>(d) : enc_form<f16, false>(d);
-}
+AttnEncForm attn_enc_form_f16(uint32_t d, int form) { return enc_form<f16>(d, form); }
 
 }  // namespace di
 
@@ -78,8 +76,9 @@ extern "C" int32_t di_attn_encoder(di_ctx* ctx, const di_heads* q, const di_head
   const uint64_t rows = (uint64_t)Sq * a.G;
   a.prows = rows * B * Hk;
   const bool f32 = dt == DI_F32;
-  const bool few = rows <= 16;
-  const AttnEncForm form = f32 ? attn_enc_form_f32(d, few) : attn_enc_form_f16(d, few);
+  int kind = rows <= 16 ? ENC_FEW : rows <= 64 ? ENC_MID : ENC_MANY;
+  if (bias && !enc_bias_ok(d, kind)) kind = ENC_MID;
+  const AttnEncForm form = f32 ? attn_enc_form_f32(d, kind) : attn_enc_form_f16(d, kind);
   const uint32_t R = form.rows, KT = form.tile, WK = form.groups;
   const uint64_t blocks = (rows + R - 1) / R, groups = blocks * B * Hk;
   DI_REQUIRE(rows < 1ull << 31 && groups < 1ull << 24, DI_EUNSUPPORTED, "%s: %llu rows per key head, %llu workgroups",
@@ -102,8 +101,8 @@ extern "C" int32_t di_attn_encoder(di_ctx* ctx, const di_heads* q, const di_head
     a.part_o = (float*)ws;
     a.part_ml = (float*)((char*)ws + ob);
   }
-  if (f32) launch_attn_enc_f32(a, B, few, ctx->stream);
-  else launch_attn_enc_f16(a, B, few, ctx->stream);
+  if (f32) launch_attn_enc_f32(a, B, kind, ctx->stream);
+  else launch_attn_enc_f16(a, B, kind, ctx->stream);
   if (ws) pool_release(ctx, ws, cap);
   DI_LAUNCH_CHECK();
   return DI_OK;

@@ -3,12 +3,10 @@
 
 namespace di {
 
-void launch_attn_enc_f32(const AttnEncArgs& a, uint32_t B, bool few, hipStream_t s) {
-  launch_enc<float>(a, B, few, s);
+void launch_attn_enc_f32(const AttnEncArgs& a, uint32_t B, int form, hipStream_t s) {
+  launch_enc<float>(a, B, form, s);
 }
 
-AttnEncForm attn_enc_form_f32(uint32_t d, bool few) {
-  return few ? enc_form<float, true>(d) : enc_form<float, false>(d);
-}
+AttnEncForm attn_enc_form_f32(uint32_t d, int form) { return enc_form<float>(d, form); }
 
 }  // namespace di
