@@ -37,7 +37,7 @@
 // of wavefronts walk different tiles of the same rows and are merged through
 // LDS.  Forms: many rows, WM = 4 and QG = 2 (two groups share every fragment
 // read); up to 64 rows, WM = 4 and QG = 1; few rows (a token, a handful of
-// latents), WM = 1 and WK = 4, so that every wavefront streams keys of its own.
+// latents), WM = 1 and WK = 2 to 8, so that every wavefront streams keys of its own.
 // Where the rows still leave CUs idle the keys are split over workgroups as
 // well and k_attn_enc_merge joins the parts.
 #pragma once
@@ -82,6 +82,14 @@ __device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, unsigned ch
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)p, 16, off, 0, 0, 0);
 }
 
+// Orders LDS accesses of one wavefront's lanes, which the hardware keeps in
+// order by itself, for the compiler.
+__device__ __forceinline__ void enc_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // lanes l, l^16, l^32, l^48 hold the same row
 __device__ __forceinline__ float enc_max4(float x) {
   auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -105,13 +113,15 @@ struct EncShape {
   // chunks of an LDS row: a power of two
   static constexpr int C0 = DK / EPC;
   static constexpr int CPR = C0 <= 4 ? 4 : C0 <= 8 ? 8 : C0 <= 16 ? 16 : C0 <= 32 ? 32 : 64;
-  // keys per tile: K and V tile of at most 32 KiB together (16 KiB for few rows)
-  static constexpr int KT = FEW ? (CPR <= 16 ? 32 : F32 ? 16 : 32)
-                                : (CPR <= 16 ? 64 : CPR == 32 ? 32 : 16);
+  // Keys per tile: 32 where the wavefronts share out whole loads, 16 where an
+  // fp32 tile would pass 16 KiB.  (64 at up to 128 channels: 2 x 16 x 8192 rows
+  // over 512 keys 81.3 us at 128 channels and 49.8 at 64, 80.3 and 45.8 so, with
+  // room for more workgroups on a CU.)
+  static constexpr int KT = CPR == 4 && !FEW ? 64 : F32 && CPR >= (FEW ? 32 : 64) ? 16 : 32;
   static constexpr int TILE = KT * CPR * 16;  // bytes of a K (V) tile
   static constexpr int WM = FEW ? 1 : 4;
-  // four wavefronts' buffers while they fit the 160 KiB of LDS
-  static constexpr int WK = FEW ? (TILE * 4 * 4 <= 128 * 1024 ? 4 : 2) : 1;
+  // as many wavefronts' buffers as fit the 160 KiB of LDS
+  static constexpr int WK = !FEW ? 1 : TILE * 4 * 8 <= 128 * 1024 ? 8 : TILE * 4 * 4 <= 128 * 1024 ? 4 : 2;
   // two row groups where their accumulators leave room for two wavefronts a SIMD
   static constexpr int QG = FORM == ENC_MANY && !F32 && DK <= 128 ? 2 : 1;
   static constexpr int ROWS = WM * QG * 16;
@@ -543,11 +553,20 @@ void k_attn_enc(AttnEncArgs a) {
     m[0] = mx;
   }
 
-  // lane (r, g) holds channels 16 dt + 4 g .. + 3 of its rows
+  // lane (r, g) holds channels 16 dt + 4 g .. + 3 of its rows.  fp16 outputs
+  // of several wavefronts go through a strip of LDS each (the tiles' memory is
+  // free by then), so that a wavefront writes rows of whole 16-byte vectors and
+  // not 32 bytes of sixteen rows at a time (2 x 16 x 8192 rows of 128 over 64
+  // keys: 40.5 -> 33.9 us).
+  constexpr bool SWAP = !F32 && WM > 1;
+  constexpr int SP = DK * 2 + 16;  // bytes between a strip's rows
+  static_assert(!SWAP || 4 * 16 * SP <= Sh::LDS, "the strips fit the buffers");
+  unsigned char* const strip = smem + wm * 16 * SP;
+  if constexpr (SWAP) __syncthreads();
 #pragma unroll
   for (int i = 0; i < QG; i++) {
-    if (!live[i]) continue;
     if (a.splits > 1) {
+      if (!live[i]) continue;
       const uint64_t prow = (uint64_t)split * a.prows + (uint64_t)hb * a.rows + row[i];
       float* dst = a.part_o + prow * a.d;
 #pragma unroll
@@ -557,13 +576,34 @@ void k_attn_enc(AttnEncArgs a) {
       continue;
     }
     const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
-    T* dst = (T*)a.o + b * a.bo + qh[i] * a.ho + (uint64_t)qi_[i] * a.ldo;
+    if constexpr (SWAP) {
 #pragma unroll
-    for (int dt = 0; dt < NDT; dt++) {
-      if (dt * 16 + g * 4 >= a.d) continue;
-      const f32x4 v = o[i][dt] * inv;
-      if constexpr (F32) *(f32x4*)(dst + dt * 16 + g * 4) = v;
-      else *(f16x4*)(dst + dt * 16 + g * 4) = f16x4{(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3]};
+      for (int dt = 0; dt < NDT; dt++) {
+        const f32x4 v = o[i][dt] * inv;
+        *(f16x4*)(strip + r * SP + dt * 32 + g * 8) = f16x4{(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3]};
+      }
+      enc_lds_fence();
+      constexpr int CH = DK / 8;  // 16-byte chunks of a row
+      const uint32_t row0 = mb * Sh::ROWS + (wm * QG + i) * 16;
+#pragma unroll
+      for (int it = 0; it < 16 * CH / 64; it++) {
+        const uint32_t x = it * 64 + lane, rr = x / CH, c = x % CH, row = row0 + rr;
+        const f16x8 v = *(const f16x8*)(strip + rr * SP + c * 16);
+        if (row >= a.rows || c * 8 >= a.d) continue;
+        const uint32_t qi = a.G == 1 ? row : row / a.G, qh = h * a.G + (row - qi * a.G);
+        *(f16x8*)((f16*)a.o + b * a.bo + qh * a.ho + (uint64_t)qi * a.ldo + c * 8) = v;
+      }
+      enc_lds_fence();
+    } else {
+      if (!live[i]) continue;
+      T* dst = (T*)a.o + b * a.bo + qh[i] * a.ho + (uint64_t)qi_[i] * a.ldo;
+#pragma unroll
+      for (int dt = 0; dt < NDT; dt++) {
+        if (dt * 16 + g * 4 >= a.d) continue;
+        const f32x4 v = o[i][dt] * inv;
+        if constexpr (F32) *(f32x4*)(dst + dt * 16 + g * 4) = v;
+        else *(f16x4*)(dst + dt * 16 + g * 4) = f16x4{(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3]};
+      }
     }
   }
 }

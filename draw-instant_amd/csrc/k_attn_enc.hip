@@ -1,5 +1,6 @@
 // Attention to an encoder's states: the fp16 instantiations of k_attn_enc.h,
 // the choice of form and key split, and the C ABI (di_attn_encoder).
+#include <algorithm>
 #include <cmath>
 
 #include "di_views.h"
@@ -76,8 +77,15 @@ extern "C" int32_t di_attn_encoder(di_ctx* ctx, const di_heads* q, const di_head
   const uint64_t rows = (uint64_t)Sq * a.G;
   a.prows = rows * B * Hk;
   const bool f32 = dt == DI_F32;
-  int kind = rows <= 16 ? ENC_FEW : rows <= 64 ? ENC_MID : ENC_MANY;
-  if (bias && !enc_bias_ok(d, kind)) kind = ENC_MID;
+  // Two row groups a wavefront where that still leaves two workgroups a CU and,
+  // with over 64 channels, keys enough to pay for the longer start: 2 x 16 heads
+  // of 8192 x 512 keys of 128 80 us and with one group 87, 256 keys 48.8 and
+  // 49.7, 154 keys 41.2 and 38.1; 8 heads of 4096 x 77 keys of 40 6.8 and 7.6; 24
+  // heads of 1000 x 512 keys of 128, 192 workgroups, 15.9 and 13.9.
+  int kind = rows <= 16 ? ENC_FEW : ENC_MID;
+  if (!f32 && rows > 64 && (d <= 64 || (d <= 128 && Skv > 192)) && enc_bias_ok(d, bias ? ENC_MANY : ENC_MID) &&
+      (rows + 127) / 128 * B * Hk >= 2ull * ctx->num_cus)
+    kind = ENC_MANY;
   const AttnEncForm form = f32 ? attn_enc_form_f32(d, kind) : attn_enc_form_f16(d, kind);
   const uint32_t R = form.rows, KT = form.tile, WK = form.groups;
   const uint64_t blocks = (rows + R - 1) / R, groups = blocks * B * Hk;
@@ -85,12 +93,21 @@ extern "C" int32_t di_attn_encoder(di_ctx* ctx, const di_heads* q, const di_head
              fn, (unsigned long long)rows, (unsigned long long)groups);
   a.rows = (uint32_t)rows;
   a.blocks = (uint32_t)blocks;
-  // key ranges: enough workgroups for two a CU, each of at least four tiles per key group
-  const uint64_t n_tiles = (Skv + KT - 1) / KT, most = n_tiles / (4 * WK);
-  uint64_t sp = 2ull * ctx->num_cus / groups;
-  sp = sp < most ? sp : most;
-  sp = sp < 64 ? sp : 64;
-  a.splits = sp < 2 ? 1 : (uint32_t)sp;
+  // Key ranges, at most a workgroup per CU and two to four tiles each, by what
+  // they save (a tile takes a wavefront 0.5 us on a CU of its own) less what the
+  // merge costs (3 us and the parts' bytes at 4 TB/s).  16 heads' single tokens over
+  // 8000 keys of 64 18.0 us in one piece, 8.4 in 16 ranges; 8 heads of 64 queries
+  // over 16384 keys of 128 281, 20.7 in 32 ranges, 23.5 in 64; 64 heads' tokens
+  // over 1500 keys, six tiles a wavefront, 7.0 and in four ranges 8.2.
+  const uint64_t n_tiles = (Skv + KT - 1) / KT;
+  uint64_t most = n_tiles / (kind == ENC_FEW ? 2 * WK : 4);
+  most = std::min<uint64_t>({most, ctx->num_cus / groups, 64});
+  a.splits = 1;
+  double best = 0.0;
+  for (uint32_t sp = 2; sp <= most; sp++) {
+    const double gain = (double)n_tiles / WK * (1.0 - 1.0 / sp) * 0.5 - 3.0 - (double)sp * a.prows * d * 8 / 4e6;
+    if (gain > best) best = gain, a.splits = sp;
+  }
   DI_HIP(hipSetDevice(ctx->device));
   void* ws = nullptr;
   uint64_t cap = 0;

@@ -232,3 +232,21 @@ def test_matches_cross_attention(dev, rng):
     assert (np.abs(got.astype(np.float64) - ref) <= 2 * bound.transpose(0, 2, 1, 3)).all()
     for b in bufs:
         b.destroy()
+
+
+@pytest.mark.parametrize("d,Skv,kind", [(32, 45, "bias"), (40, 77, "lens"), (64, 300, "bias"), (64, 33, "none"),
+                                        (72, 200, "lens"), (96, 256, "none"), (128, 300, "lens"), (128, 193, "bias")])
+def test_many_rows(dev, rng, d, Skv, kind):
+    """Grids that fill the chip twice over: two row groups a wavefront, the
+    last one ragged, heads shared by three queries each."""
+    B, Hk, G, Sq = 4, 64, 3, 67  # two blocks of 128 rows, 512 workgroups
+    c = Case(dev, rng, B, Hk * G, Hk, Sq, Skv, d, F16, stacked=True)
+    lens = [Skv, 1, Skv - 30, 33] if kind == "lens" else None
+    bias = None
+    if kind == "bias":
+        bias = rng.standard_normal((B, 1, Sq, Skv)).astype(np.float32)
+        bias[rng.random(bias.shape) < 0.3] = -np.inf
+        bias[:, :, 5] = -np.inf
+    k, v = c.kv()
+    got = c.run(lens=lens, bias=bias, bias_strides=dict(batch=Sq * Skv, query=Skv))
+    check(got, *attention(c.q, k, v, lens, bias), f"many rows d={d} {kind}")
