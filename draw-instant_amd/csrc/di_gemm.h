@@ -226,6 +226,11 @@ bool gemm_lnfold_ok(const GemmArgs& g, int elem, int tile_cfg);
 void launch_lora_down(const void* x, const void* down, const float* scale, const int32_t* ids, void* t,
                       uint32_t M, uint32_t K, uint32_t n, uint32_t rank, uint32_t ld, uint32_t run,
                       int elem, int num_cus, hipStream_t s);
+// Few fp16 rows: d[m][n] = sum_r t[m][r] up[a][n][r] in fp32 with t as above
+// (rounded to fp16), zero for rows without an adapter.
+void launch_lora_rows(const void* x, const void* down, const void* up, const float* scale, const int32_t* ids,
+                      float* d, uint32_t M, uint32_t N, uint32_t K, uint32_t n, uint32_t rank, uint32_t run,
+                      hipStream_t s);
 // OIHW (any dtype) -> OHWI fp16 with optional zero channel padding Cin -> Cin_pad.
 void launch_repack_oihw_ohwi(hipStream_t s, const void* w, int wdt, void* out, uint32_t Cout,
                              uint32_t Cin, uint32_t ks, uint32_t Cin_pad);

@@ -401,19 +401,20 @@ __global__ __launch_bounds__(256, 2) void k_gemm_f32(GemmArgs g) {
 
   // adapters: k index e runs on over (adapter of the tile, rank) after the last k
   uint32_t lo_total = 0;
-  int32_t rid[LORA ? BM / 32 : 1];
+  int32_t rid[LORA ? BM / 32 : 1], lo_cnt = 0;
+  LoraRows<LORA ? BM : 1> lo_rows(g, m0, sLo);
   if constexpr (LORA) {
     if (split == 0) {
-      if (wave == 0) lora_tile<BM>(g, m0, sLo);
-#pragma unroll
-      for (int i = 0; i < BM / 32; i++) rid[i] = lora_id(g, m0 + (threadIdx.x >> 3) + 32 * i);
+      lo_rows.load(rid, threadIdx.x >> 3, 32);
+      lo_rows.take(rid, threadIdx.x >> 3, 32, wave == 0);
       __syncthreads();
-      lo_total = (uint32_t)sLo.n * g.lo_ld;
+      lo_cnt = lo_rows.count();
+      lo_total = (uint32_t)lo_cnt * g.lo_ld;
     }
   }
   auto load_lora = [&](uint32_t e0, F32Tile<BM>& ta, F32Tile<BN>& tb) {
     const uint32_t e = e0 + (threadIdx.x & 7) * 4, slot = e / g.lo_ld, rr = e - slot * g.lo_ld;
-    const int32_t ad = slot < (uint32_t)sLo.n ? sLo.ad[slot] : -2;
+    const int32_t ad = lo_rows.slot(slot, lo_cnt);
 #pragma unroll
     for (int i = 0; i < BM / 32; i++) {
       f32x4 v = {0.f, 0.f, 0.f, 0.f};

@@ -228,44 +228,106 @@ __device__ __forceinline__ void epi_math8(const GemmArgs& g, float* x, const f32
 // GEMM's allocation.
 enum { EX_NONE = 0, EX_ROWSTATS = 1, EX_LNFOLD = 2, EX_LORA = 3 };
 
-// The adapters that a tile's rows name (g.lo_*), each once, in order of first
-// appearance: `n` of them.
+// The adapters that a tile's rows m0 .. m0 + BM - 1 name (g.lo_*), each once, and
+// the one of each row.  Where a run of rows is as long as a tile the tile meets
+// two at most: two scalar loads, and a row's adapter is a comparison (reading an
+// id per row costs the 10240 workgroups of 32768 x 2560 x 320 14 us).  Else the
+// rows' ids are read one by one and the distinct ones listed in LDS.
 template <int BM>
 struct LoraTile {
   int32_t ad[BM];
   int32_t n;
 };
 
-// Adapter of row m, -1 where it has none.
-__device__ __forceinline__ int32_t lora_id(const GemmArgs& g, uint32_t m) {
-  if (m >= g.M) return -1;
-  const int32_t id = g.lo_ids[m / g.lo_run];
-  return (uint32_t)id < g.lo_n ? id : -1;
-}
-
-// Fills `lo` for rows m0 .. m0 + BM - 1: one wavefront, no barrier.
 template <int BM>
-__device__ __forceinline__ void lora_tile(const GemmArgs& g, uint32_t m0, LoraTile<BM>& lo) {
-  constexpr int NI = (BM + 63) / 64;
-  const uint32_t lane = threadIdx.x & 63;
-  int32_t id[NI];
-#pragma unroll
-  for (int i = 0; i < NI; i++) id[i] = lane + 64 * i < BM ? lora_id(g, m0 + lane + 64 * i) : -1;
-  int32_t n = 0;
-#pragma unroll
-  for (int i = 0; i < NI; i++) {
-    uint64_t todo;
-    while ((todo = __builtin_amdgcn_ballot_w64(id[i] >= 0)) != 0) {
-      const int32_t a = __builtin_amdgcn_readlane(id[i], __builtin_ctzll(todo));
-      if (lane == 0) lo.ad[n] = a;
-      n++;
-#pragma unroll
-      for (int k = i; k < NI; k++)
-        if (id[k] == a) id[k] = -1;
-    }
+struct LoraRows {
+  static constexpr int NI = (BM + 63) / 64;
+  const GemmArgs& g;
+  LoraTile<BM>& lo;
+  uint32_t m0, q0, rem;
+  bool two;
+  int32_t a0, a1;  // two: adapter of the rows before and from `cross` on, -1 none
+  uint32_t cross;
+  int32_t all[NI];
+
+  __device__ __forceinline__ LoraRows(const GemmArgs& g, uint32_t m0, LoraTile<BM>& lo) : g(g), lo(lo), m0(m0) {}
+
+  __device__ __forceinline__ int32_t valid(int32_t id) const { return (uint32_t)id < g.lo_n ? id : -1; }
+
+  // Id of row m0 + r (rows past the problem: of its last one), at lo_ids[q0 +
+  // (rem + r) / run].  The quotient of two numbers below 2^24 by the hardware's
+  // reciprocal is off by one at most.
+  __device__ __forceinline__ int32_t load_row(uint32_t r) const {
+    const uint32_t x = rem + min(r, g.M - 1 - m0);
+    uint32_t q = (uint32_t)((float)x * __builtin_amdgcn_rcpf((float)g.lo_run));
+    const int32_t left = (int32_t)(x - q * g.lo_run);
+    q = left < 0 ? q - 1 : left >= (int32_t)g.lo_run ? q + 1 : q;
+    return g.lo_ids[q0 + q];
   }
-  if (lane == 0) lo.n = n;
-}
+
+  __device__ __forceinline__ void load_two() {
+    q0 = __builtin_amdgcn_readfirstlane(m0 / g.lo_run);
+    rem = m0 - q0 * g.lo_run;
+    two = g.lo_run >= (uint32_t)BM;
+    cross = g.lo_run - rem;
+    a0 = two ? g.lo_ids[q0] : -1;
+    a1 = two && cross < min((uint32_t)BM, g.M - m0) ? g.lo_ids[q0 + 1] : a0;
+  }
+  // Issues the ids' loads: rid[i] for this thread's rows row0 + i * step.
+  template <int N>
+  __device__ __forceinline__ void load(int32_t (&rid)[N], uint32_t row0, uint32_t step) {
+    load_two();
+    if (two) return;
+#pragma unroll
+    for (int i = 0; i < N; i++) rid[i] = load_row(row0 + i * step);
+#pragma unroll
+    for (int i = 0; i < NI; i++) all[i] = load_row((threadIdx.x & 63) + 64 * i);
+  }
+
+  // Turns them into adapters; wavefront `lists` writes the list (no barrier).
+  template <int N>
+  __device__ __forceinline__ void take(int32_t (&rid)[N], uint32_t row0, uint32_t step, bool lists) {
+    if (two) {
+      a0 = valid(a0);
+      a1 = valid(a1);
+#pragma unroll
+      for (int i = 0; i < N; i++) rid[i] = row0 + i * step < cross ? a0 : a1;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++)
+      rid[i] = row0 + i * step < (uint32_t)BM && m0 + row0 + i * step < g.M ? valid(rid[i]) : -1;
+    if (two || !lists) return;
+    const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < NI; i++)
+      all[i] = lane + 64 * i < BM && m0 + lane + 64 * i < g.M ? valid(all[i]) : -1;
+    int32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+      uint64_t todo;
+      while ((todo = __builtin_amdgcn_ballot_w64(all[i] >= 0)) != 0) {
+        const int32_t a = __builtin_amdgcn_readlane(all[i], __builtin_ctzll(todo));
+        if (lane == 0) lo.ad[n] = a;
+        n++;
+#pragma unroll
+        for (int k = i; k < NI; k++)
+          if (all[k] == a) all[k] = -1;
+      }
+    }
+    if (lane == 0) lo.n = n;
+  }
+
+  // Number of adapters, and the one in a slot (-2: none; after a barrier).
+  __device__ __forceinline__ int32_t count() const {
+    if (two) return (a0 >= 0) + (a1 >= 0 && a1 != a0);
+    return __builtin_amdgcn_readfirstlane(lo.n);
+  }
+  __device__ __forceinline__ int32_t slot(uint32_t s, int32_t n) const {
+    if (s >= (uint32_t)n) return -2;
+    if (two) return s == 0 && a0 >= 0 ? a0 : a1;
+    return lo.ad[s];
+  }
+};
 
 // Barrier for hand-offs through LDS inside a workgroup: waits for the
 // wave's LDS operations only and meets the other waves, leaving global
@@ -1109,28 +1171,30 @@ __global__ __launch_bounds__(64 * WGM * WGN * KS) void k_gemm(GemmArgs g) {
   }
   }
 
-  // Adapters: the tile's k index goes on over (adapter of the tile, rank), the
-  // A operand being the row's own inner products lo_t under its own adapter
-  // and zero under the others; a stage may hold several adapters.  One split
-  // takes them.
+  // Adapters (one split takes them): the tile's k index goes on over (adapter of
+  // the tile, rank), the A operand being the row's own inner products lo_t under
+  // its own adapter and zero under the others; a stage may hold several
+  // adapters.  After the pipeline: taken into its register ring, by a scalar
+  // choice of descriptor per load, they slowed every stage of it (32768 x 2560 x
+  // 320 without any adapter 120 -> 131 us, with rank 64 148 either way).
   if constexpr (EX == EX_LORA) {
     if (split == 0) {
-      if (wave == 0) lora_tile<BM>(g, m0, sLo);
-      int32_t rid[NVA];
-#pragma unroll
-      for (int i = 0; i < NVA; i++) rid[i] = a_ld ? lora_id(g, m0 + (tid + i * NT) / VPR) : -1;
+      LoraRows<BM> lo_rows(g, m0, sLo);
+      int32_t lo_rid[NVA];
+      lo_rows.load(lo_rid, tid / VPR, NT / VPR);
+      lo_rows.take(lo_rid, tid / VPR, NT / VPR, wave == NT / 64 - 1);
       __syncthreads();
-      const int32_t n_ad = sLo.n;
-      const uint32_t total = (uint32_t)n_ad * g.lo_ld;
+      const int32_t lo_cnt = lo_rows.count();
+      const uint32_t total = (uint32_t)lo_cnt * g.lo_ld;
       const bool whole = g.lo_rank == g.lo_ld;
       for (uint32_t e0 = 0; e0 < total; e0 += BK) {
         const uint32_t e = e0 + kc * KV, slot = e / g.lo_ld, rr = e - slot * g.lo_ld;
-        const int32_t ad = slot < (uint32_t)n_ad ? sLo.ad[slot] : -2;
+        const int32_t ad = lo_rows.slot(slot, lo_cnt);
         Stage st;
 #pragma unroll
         for (int i = 0; i < NVA; i++) {
           st.a[i] = zero_vec<T>();
-          if (rid[i] == ad)
+          if (lo_rid[i] == ad)
             st.a[i] = *(const typename MT::vec*)((const T*)g.lo_t +
                                                  (uint64_t)(m0 + (tid + i * NT) / VPR) * g.lo_ld + rr);
         }
