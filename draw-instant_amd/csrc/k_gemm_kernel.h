@@ -1112,78 +1112,22 @@ __global__ __launch_bounds__(64 * WGM * WGN * KS) void k_gemm(GemmArgs g) {
       if (tid < BN) sLn[2 * BM + tid] = ln_col;
     }
   };
-  Stage r0, r1;
-  if constexpr (FAST) {
-    static_assert(D % 2 == 0, "even ring depth: LDS buffer = stage parity");
-    Stage r[D];
-    if (n_stages > 0) {
-#pragma unroll
-      for (int j = 0; j < D; j++) load(j, r[j]);
-      ln_issue();
-      store_stage(0, r[0]);
-      load(D, r[0]);
-      ln_publish();  // after stage D's loads are issued: its wait covers stage 1 only
-      __syncthreads();
-      // steady state: whole rounds of D stages, no conditions (a conditional
-      // compute makes the compiler copy the accumulators around it)
-      int s0 = 0;
-      for (; s0 + D <= n_stages; s0 += D) {
-#pragma unroll
-        for (int j = 0; j < D; j++) {
-          store_stage((j + 1) & 1, r[(j + 1) % D]);
-          load(s0 + j + 1 + D, r[(j + 1) % D]);
-          // issue the loads here, not after the MFMAs (the scheduler would
-          // otherwise sink them and shorten the prefetch distance)
-          __builtin_amdgcn_sched_barrier(0);
-          compute(j & 1);
-          __syncthreads();
-        }
-      }
-      // tail: the last n_stages % D stages (stage s0 + j in LDS buffer j & 1)
-      const int rem = n_stages - s0;
-#pragma unroll
-      for (int j = 0; j + 1 < D; j++) {
-        if (j < rem) {
-          if (j + 1 < rem) store_stage((j + 1) & 1, r[(j + 1) % D]);
-          compute(j & 1);
-          __syncthreads();
-        }
-      }
-    }
-  } else {
-  if (n_stages > 0) {
-    load(0, r0);
-    store_stage(0, r0);
-  }
-  if (n_stages > 1) load(1, r1);
-  if (n_stages > 2) load(2, r0);
-  __syncthreads();
-  for (int s = 0; s < n_stages; s += 2) {
-    compute(0);
-    if (s + 1 < n_stages) store_stage(1, r1);
-    __syncthreads();
-    if (s + 3 < n_stages) load(s + 3, r1);
-    if (s + 1 >= n_stages) break;
-    compute(1);
-    if (s + 2 < n_stages) store_stage(0, r0);
-    __syncthreads();
-    if (s + 4 < n_stages) load(s + 4, r0);
-  }
-  }
-
-  // Adapters (one split takes them): the tile's k index goes on over (adapter of
-  // the tile, rank), the A operand being the row's own inner products lo_t under
-  // its own adapter and zero under the others; a stage may hold several
-  // adapters.  After the pipeline: taken into its register ring, by a scalar
-  // choice of descriptor per load, they slowed every stage of it (32768 x 2560 x
-  // 320 without any adapter 120 -> 131 us, with rank 64 148 either way).
-  if constexpr (EX == EX_LORA) {
-    if (split == 0) {
+  // Adapters (one split takes them): the tile's k index runs over (adapter of the
+  // tile, rank) as well, the A operand being the row's own inner products lo_t
+  // under its own adapter and zero under the others; a stage may hold several
+  // adapters.  These stages come first: their ids' and operands' round trips then
+  // overlap those of the first main stages, whose loads are issued
+  // before (4096 x 640 x 640 with rank 32 18.7 us, after the main loop 19.1).  Taken into the ring of register stages, by a scalar choice of
+  // descriptor per load, they slowed every stage of it (32768 x 2560 x 320
+  // without any adapter 120 -> 131 us).
+  auto lora_stages = [&]() {
+    if constexpr (EX == EX_LORA) {
+      if (split != 0) return;
       LoraRows<BM> lo_rows(g, m0, sLo);
       int32_t lo_rid[NVA];
       lo_rows.load(lo_rid, tid / VPR, NT / VPR);
       lo_rows.take(lo_rid, tid / VPR, NT / VPR, wave == NT / 64 - 1);
-      __syncthreads();
+      if (!lo_rows.two) __syncthreads();
       const int32_t lo_cnt = lo_rows.count();
       const uint32_t total = (uint32_t)lo_cnt * g.lo_ld;
       const bool whole = g.lo_rank == g.lo_ld;
@@ -1219,6 +1163,66 @@ __global__ __launch_bounds__(64 * WGM * WGN * KS) void k_gemm(GemmArgs g) {
         __syncthreads();
       }
     }
+  };
+  Stage r0, r1;
+  if constexpr (FAST) {
+    static_assert(D % 2 == 0, "even ring depth: LDS buffer = stage parity");
+    Stage r[D];
+    if (n_stages > 0) {
+#pragma unroll
+      for (int j = 0; j < D; j++) load(j, r[j]);
+      lora_stages();
+      ln_issue();
+      store_stage(0, r[0]);
+      load(D, r[0]);
+      ln_publish();  // after stage D's loads are issued: its wait covers stage 1 only
+      __syncthreads();
+      // steady state: whole rounds of D stages, no conditions (a conditional
+      // compute makes the compiler copy the accumulators around it)
+      int s0 = 0;
+      for (; s0 + D <= n_stages; s0 += D) {
+#pragma unroll
+        for (int j = 0; j < D; j++) {
+          store_stage((j + 1) & 1, r[(j + 1) % D]);
+          load(s0 + j + 1 + D, r[(j + 1) % D]);
+          // issue the loads here, not after the MFMAs (the scheduler would
+          // otherwise sink them and shorten the prefetch distance)
+          __builtin_amdgcn_sched_barrier(0);
+          compute(j & 1);
+          __syncthreads();
+        }
+      }
+      // tail: the last n_stages % D stages (stage s0 + j in LDS buffer j & 1)
+      const int rem = n_stages - s0;
+#pragma unroll
+      for (int j = 0; j + 1 < D; j++) {
+        if (j < rem) {
+          if (j + 1 < rem) store_stage((j + 1) & 1, r[(j + 1) % D]);
+          compute(j & 1);
+          __syncthreads();
+        }
+      }
+    }
+  } else {
+  lora_stages();
+  if (n_stages > 0) {
+    load(0, r0);
+    store_stage(0, r0);
+  }
+  if (n_stages > 1) load(1, r1);
+  if (n_stages > 2) load(2, r0);
+  __syncthreads();
+  for (int s = 0; s < n_stages; s += 2) {
+    compute(0);
+    if (s + 1 < n_stages) store_stage(1, r1);
+    __syncthreads();
+    if (s + 3 < n_stages) load(s + 3, r1);
+    if (s + 1 >= n_stages) break;
+    compute(1);
+    if (s + 2 < n_stages) store_stage(0, r0);
+    __syncthreads();
+    if (s + 4 < n_stages) load(s + 4, r0);
+  }
   }
 
   // ---- epilogue ----
