@@ -205,7 +205,7 @@ int32_t di_linear_lora(di_ctx* ctx, di_handle X, di_handle W, di_handle bias, co
   GemmArgs g;
   int rc = linear_args(ctx, fn, X, W, bias, R, Y, M, N, K, act, dt, g);
   if (rc) return rc;
-  DI_REQUIRE(Y != X && Y != W, DI_EINVAL, "%s: Y is an operand", fn);
+  DI_REQUIRE(Y != X && Y != W && (!bias || Y != bias), DI_EINVAL, "%s: Y is an operand", fn);
   DI_REQUIRE(lora->n && lora->rank && lora->rows_per_id, DI_EINVAL, "%s: zero dimension (n=%u rank=%u rows_per_id=%u)",
              fn, lora->n, lora->rank, lora->rows_per_id);
   DI_REQUIRE(lora->rank <= 256, DI_EUNSUPPORTED, "%s: rank %u above 256", fn, lora->rank);

@@ -288,7 +288,7 @@ typedef struct {
  * The scaled inner products X down^T are held in dtype between the two
  * products, as activations are; every sum is fp32.  The stack must be finite:
  * rows of one tile are multiplied with each other's adapters by zeros.  Y may
- * be R, not X. */
+ * be R and no other operand. */
 int32_t di_linear_lora(di_ctx* ctx, di_handle X, di_handle W, di_handle bias,
                        const di_lora* lora, di_handle R, di_handle Y, uint32_t M, uint32_t N,
                        uint32_t K, int32_t act, int32_t dtype);

@@ -200,6 +200,7 @@ static void lora() {
   REFUSE(DI_EHANDLE, "handle", c.lo.scale = 4321);
   REFUSE(DI_EINVAL, "Y is an operand", c.N = 24; c.y = c.x);
   REFUSE(DI_EINVAL, "Y is an operand", c.y = c.w);
+  REFUSE(DI_EINVAL, "Y is an operand", c.M = 1; c.lo.rows_per_id = 1; c.y = c.b);
   REFUSE(DI_EINVAL, "Y is an operand", c.y = c.lo.up; c.M = 1; c.lo.rows_per_id = 1);
 #undef REFUSE
   expect(di_linear_lora(&ctx, x, w, b, nullptr, 0, y, 10, 32, 24, 0, 1), DI_EINVAL, "null adapters", "null adapters");
