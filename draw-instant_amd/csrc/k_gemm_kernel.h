@@ -1116,10 +1116,10 @@ __global__ __launch_bounds__(64 * WGM * WGN * KS) void k_gemm(GemmArgs g) {
   // tile, rank) as well, the A operand being the row's own inner products lo_t
   // under its own adapter and zero under the others; a stage may hold several
   // adapters.  These stages come first: their ids' and operands' round trips then
-  // overlap those of the first main stages, whose loads are issued
-  // before (4096 x 640 x 640 with rank 32 18.7 us, after the main loop 19.1).  Taken into the ring of register stages, by a scalar choice of
-  // descriptor per load, they slowed every stage of it (32768 x 2560 x 320
-  // without any adapter 120 -> 131 us).
+  // overlap those of the first main stages, whose loads are issued before (4096 x
+  // 640 x 640 with rank 32 18.7 us, after the main loop 19.1).  Taken into the ring
+  // of register stages, by a scalar choice of descriptor per load, they slowed every
+  // stage of it (32768 x 2560 x 320 without any adapter 120 -> 131 us).
   auto lora_stages = [&]() {
     if constexpr (EX == EX_LORA) {
       if (split != 0) return;
