@@ -677,7 +677,7 @@ __device__ __forceinline__ void gemm_tile_stats(const GemmArgs& g, const float* 
   }
 }
 
-// The argument block (GemmArgs, 328 bytes: six scalar-cache lines) in one
+// The argument block (GemmArgs, 384 bytes: six scalar-cache lines) in one
 // round trip at entry, instead of three serialised misses before the first
 // operand load.
 __device__ __forceinline__ void args_warm(const GemmArgs& g) { kernarg_warm(g); }
