@@ -21,6 +21,7 @@ struct AttnEncArgs {
   uint32_t rows;    // Sq * G: query rows of one key head
   uint32_t blocks;  // row blocks per key head
   uint32_t splits;  // key ranges
+  uint32_t heads_first;  // order of the workgroups, with a bias
   uint64_t prows;   // rows of the whole call: B * Hk * rows
   float scale_log2;
   float* part_o;   // [splits][prows][d], splits > 1
@@ -30,9 +31,6 @@ struct AttnEncArgs {
 // The three forms (see k_attn_enc.h): rows per workgroup, keys per tile and key
 // groups inside a workgroup.
 enum { ENC_FEW = 0, ENC_MID = 1, ENC_MANY = 2 };
-// Whether a form is built with a bias: two row groups with one and over 64
-// channels do not fit the registers (154 spilled at 128).
-constexpr bool enc_bias_ok(uint32_t d, int form) { return form != ENC_MANY || d <= 64; }
 struct AttnEncForm {
   int rows, tile, groups;
 };

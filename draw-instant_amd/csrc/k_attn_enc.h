@@ -29,9 +29,19 @@
 // are padded to DK channels in registers and to a power of two of chunks in LDS;
 // chunks past d and keys past the length are never read from memory and land
 // as zeros.  The loop is pipelined over tiles: the scores of tile t + 1 are
-// multiplied between the exponentials of tile t, so that a wavefront has
-// matrix and vector work at once, then tile t's probabilities meet its values.
+// multiplied before the exponentials of tile t, which do not wait for them, then
+// tile t's probabilities meet its values; of two wavefronts on a SIMD one then
+// has matrix work while the other has vector work.  (Matrix and exponential
+// instructions of one wavefront in alternation were slower: 2 x 16 x 8190 rows of
+// 128 over 512 keys 88.8 -> 93.2 us, 8 heads of 2048 x 1024 of 256 27.9 -> 34.3.)
 // K is therefore fetched two tiles ahead and V one, each into two buffers.
+//
+// Biases.  A wavefront's tile without a value at or below kSwamped only has its
+// products with log2(e) taken; else scores and values are looked at one by one,
+// and the keys that no row sees are found by an or over the rows' bit masks: only
+// a tile with such a key has its values masked (2 x 10 heads of 2048 x 1024 keys of
+// 64, a third of the keys removed at random: 53 -> 46 us, fp32 140 -> 127; none
+// removed 43 -> 40).
 //
 // WM wavefronts share a tile, each with QG groups of 16 rows; WK such groups
 // of wavefronts walk different tiles of the same rows and are merged through
@@ -104,6 +114,18 @@ __device__ __forceinline__ float enc_sum4(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// or of the 16 lanes that hold one group's rows
+template <int CTRL>
+__device__ __forceinline__ uint32_t enc_or_dpp(uint32_t x) {
+  return x | (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
+}
+__device__ __forceinline__ uint32_t enc_or16(uint32_t x) {
+  x = enc_or_dpp<0xB1>(x);    // quad_perm 1 0 3 2
+  x = enc_or_dpp<0x4E>(x);    // quad_perm 2 3 0 1
+  x = enc_or_dpp<0x141>(x);   // row_half_mirror
+  return enc_or_dpp<0x140>(x);  // row_mirror
+}
+
 // Shapes of one instantiation.
 template <typename T, int DK, int FORM>
 struct EncShape {
@@ -154,8 +176,13 @@ void k_attn_enc(AttnEncArgs a) {
   const uint32_t T_ = gridDim.x, bid = blockIdx.x, xcd = bid & 7u, idx = bid >> 3;
   const uint32_t per = T_ >> 3, extra = T_ & 7u;
   const uint32_t w = xcd < extra ? xcd * (per + 1) + idx : extra * (per + 1) + (xcd - extra) * per + idx;
-  const uint32_t mb = w % a.blocks, rest = w / a.blocks, split = rest % a.splits, hb = rest / a.splits;
-  const uint32_t h = hb % a.Hk, b = hb / a.Hk;
+  // (heads_first: the heads of a block of rows side by side instead, as they
+  // read one bias)
+  const bool hf = BIAS && a.heads_first;
+  const uint32_t n0 = hf ? a.Hk : a.blocks, r0 = w / n0, i0 = w - r0 * n0;
+  const uint32_t n1 = hf ? a.blocks : a.splits, r1 = r0 / n1, i1 = r0 - r1 * n1;
+  const uint32_t n2 = hf ? a.splits : a.Hk, b = r1 / n2, i2 = r1 - b * n2;
+  const uint32_t mb = hf ? i1 : i0, split = hf ? i2 : i1, h = hf ? i0 : i2, hb = b * a.Hk + h;
 
   // this entry's keys; its tiles [t0, t1) of this workgroup's range and key group
   uint32_t nk = a.Skv;
@@ -331,25 +358,56 @@ void k_attn_enc(AttnEncArgs a) {
         }
     }
   };
-  // the loaded bias in log2 units and its effect on scores that do not count;
-  // whether some row of this wavefront does not see some key
-  auto apply_bias = [&](f32x4 (&s)[QG][NKT]) -> bool {
-    bool removed = false;
+  // The loaded bias becomes the current one; whether a value of the wavefront
+  // needs more than its product with log2(e).
+  auto take_bias = [&]() -> bool {
+    float low = 0.0f;
     if constexpr (BIAS) {
 #pragma unroll
       for (int i = 0; i < QG; i++)
 #pragma unroll
-        for (int kt = 0; kt < NKT; kt++)
+        for (int kt = 0; kt < NKT; kt++) {
+          bb[i][kt] = bn[i][kt];
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const float x = bn[i][kt][j];
-            removed |= x == -INFINITY;
-            if (x <= kSwamped) s[i][kt][j] = 0.0f;  // whatever the score: it may be NaN
-            // (the product of a finite bias stays finite)
-            bb[i][kt][j] = x == -INFINITY ? x : fmaxf(x * kLog2E, kLowest);
-          }
+          for (int j = 0; j < 4; j++) low = fminf(low, bb[i][kt][j]);
+        }
     }
-    return __builtin_amdgcn_ballot_w64(removed) != 0;
+    return BIAS && __builtin_amdgcn_ballot_w64(low <= kSwamped) != 0;
+  };
+  // The current bias in log2 units and its effect on scores that do not count;
+  // the keys that some row of this wavefront sees: bit 4 kt + j for key kt * 16 + 4g
+  // + j.
+  constexpr uint32_t ALL = (1u << (4 * NKT)) - 1;
+  auto apply_bias = [&](f32x4 (&s)[QG][NKT], bool low) -> uint32_t {
+    uint32_t seen = ALL;
+    if constexpr (BIAS) {
+      if (low) {
+        seen = 0;
+#pragma unroll
+        for (int i = 0; i < QG; i++) {
+          uint32_t own = 0;
+#pragma unroll
+          for (int kt = 0; kt < NKT; kt++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const float x = bb[i][kt][j];
+              const bool gone = x == -INFINITY;
+              own |= gone ? 0u : 1u << (4 * kt + j);
+              if (x <= kSwamped) s[i][kt][j] = 0.0f;  // whatever the score: it may be NaN
+              // (the product of a finite bias stays finite)
+              bb[i][kt][j] = gone ? x : fmaxf(x * kLog2E, kLowest);
+            }
+          seen |= live[i] ? own : 0u;
+        }
+        seen = enc_or16(seen);
+      } else {
+#pragma unroll
+        for (int i = 0; i < QG; i++)
+#pragma unroll
+          for (int kt = 0; kt < NKT; kt++) bb[i][kt] *= kLog2E;
+      }
+    }
+    return seen;
   };
   // raise the running maximum to this tile's where that is larger
   auto raise = [&](int i, f32x4 (&s)[QG][NKT]) {
@@ -381,8 +439,8 @@ void k_attn_enc(AttnEncArgs a) {
       }
   };
   // O^T += V^T P^T with tile t's values, in V buffer `buf`.  MASKED: the values
-  // of keys that none of this wavefront's rows sees (`seen` bit 4 kt + j: key kt *
-  // 16 + 4g + j) become zeros, as 0 * NaN would not vanish.
+  // of keys that none of this wavefront's rows sees (not in `seen`) become zeros, as
+  // 0 * NaN would not vanish.
   auto values = [&](auto buf_c, auto masked_c, uint32_t seen) {
     constexpr bool MASKED = decltype(masked_c)::value != 0;
     const unsigned char* sb = lds + decltype(buf_c)::value * TILE;
@@ -443,16 +501,14 @@ void k_attn_enc(AttnEncArgs a) {
     constexpr int cur = decltype(cur_c)::value;
     if (t + 2 < t1) fetch_k(t + 2, Int<cur>{});
     if (t + 1 < t1) fetch_v(t + 1, Int<cur ^ 1>{});
-    const bool removed = apply_bias(s);
+    const bool low = take_bias();
     if (t + 1 < t1) {
       load_bias(t + 1);
       scores(t + 1, Int<cur ^ 1>{}, sn);
-#pragma unroll
-      for (int i = 0; i < QG; i++) probs(i, s);
-    } else {
-#pragma unroll
-      for (int i = 0; i < QG; i++) probs(i, s);
     }
+    const uint32_t seen = apply_bias(s, low);
+#pragma unroll
+    for (int i = 0; i < QG; i++) probs(i, s);
 #pragma unroll
     for (int i = 0; i < QG; i++) {
       // a probability above 2^15 (or inf / NaN) shows in its lane's sum; the
@@ -463,18 +519,7 @@ void k_attn_enc(AttnEncArgs a) {
       }
       l[i] += ts[i];
     }
-    if (BIAS && removed) {
-      uint32_t seen = 0;
-#pragma unroll
-      for (int kt = 0; kt < NKT; kt++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          bool some = false;
-#pragma unroll
-          for (int i = 0; i < QG; i++) some |= live[i] && bb[BIAS ? i : 0][BIAS ? kt : 0][j] > -INFINITY;
-          const uint64_t bal = __builtin_amdgcn_ballot_w64(some);
-          seen |= (((bal >> (16 * g)) & 0xffffu) != 0 ? 1u : 0u) << (4 * kt + j);
-        }
+    if (BIAS && __builtin_amdgcn_ballot_w64(seen != ALL) != 0) {
       values(cur_c, Int<1>{}, seen);
     } else {
       values(cur_c, Int<0>{}, 0u);
@@ -681,7 +726,7 @@ template <typename T, int DK, int FORM>
 void launch_enc_form(const AttnEncArgs& a, uint32_t B, hipStream_t s) {
   typedef EncShape<T, DK, FORM> Sh;
   const dim3 grid(a.blocks * a.splits * a.Hk * B);
-  if constexpr (enc_bias_ok(DK, FORM))
+  if constexpr (FORM != ENC_MANY)
     if (a.bias) {
       k_attn_enc<T, DK, FORM, true><<<grid, Sh::NT, 0, s>>>(a);
       return;

@@ -81,9 +81,12 @@ extern "C" int32_t di_attn_encoder(di_ctx* ctx, const di_heads* q, const di_head
   // with over 64 channels, keys enough to pay for the longer start: 2 x 16 heads
   // of 8192 x 512 keys of 128 80 us and with one group 87, 256 keys 48.8 and
   // 49.7, 154 keys 41.2 and 38.1; 8 heads of 4096 x 77 keys of 40 6.8 and 7.6; 24
-  // heads of 1000 x 512 keys of 128, 192 workgroups, 15.9 and 13.9.
+  // heads of 1000 x 512 keys of 128, 192 workgroups, 15.9 and 13.9.  Not with a
+  // bias, whose values take the registers of a workgroup per CU: 2 x 10 heads of
+  // 4096 x 2048 keys of 64 168 us and with one group 156, x 77 keys 15.8 and 12.2
+  // (past 64 channels it would spill).
   int kind = rows <= 16 ? ENC_FEW : ENC_MID;
-  if (!f32 && rows > 64 && (d <= 64 || (d <= 128 && Skv > 192)) && enc_bias_ok(d, bias ? ENC_MANY : ENC_MID) &&
+  if (!f32 && rows > 64 && (d <= 64 || (d <= 128 && Skv > 192)) && !bias &&
       (rows + 127) / 128 * B * Hk >= 2ull * ctx->num_cus)
     kind = ENC_MANY;
   const AttnEncForm form = f32 ? attn_enc_form_f32(d, kind) : attn_enc_form_f16(d, kind);
@@ -107,6 +110,19 @@ extern "C" int32_t di_attn_encoder(di_ctx* ctx, const di_heads* q, const di_head
   for (uint32_t sp = 2; sp <= most; sp++) {
     const double gain = (double)n_tiles / WK * (1.0 - 1.0 / sp) * 0.5 - 3.0 - (double)sp * a.prows * d * 8 / 4e6;
     if (gain > best) best = gain, a.splits = sp;
+  }
+  if (bias && bias->head == 0) {
+    // One bias for all heads: they go side by side where the workgroups that an
+    // XCD holds then touch fewer bytes of keys, values and bias in its L2.  2 x 10
+    // heads of 4096 x 2048 keys of 64 140 us and head by head 156, 2 x 5 of 9216 x
+    // 9216 755 and 886; 24 of 1000 x 512 of 128, whose keys pass the L2 so, 22.8 and
+    // 20.1.
+    const uint64_t run = std::min<uint64_t>((groups * a.splits + 7) / 8, ctx->num_cus / 4);
+    const uint64_t kv = (uint64_t)Skv * d * 2 * dtype_size(dt);
+    const uint64_t bi = (bias->query ? std::max<uint64_t>(R / a.G, 1) : 1) * Skv * 4;
+    const uint64_t by_head = (run + blocks - 1) / blocks * kv + std::min(run, blocks * a.splits) * bi;
+    const uint64_t by_block = std::min<uint64_t>(run, Hk) * kv + (run + Hk - 1) / Hk * bi;
+    a.heads_first = by_block < by_head;
   }
   DI_HIP(hipSetDevice(ctx->device));
   void* ws = nullptr;

@@ -250,3 +250,19 @@ def test_many_rows(dev, rng, d, Skv, kind):
     k, v = c.kv()
     got = c.run(lens=lens, bias=bias, bias_strides=dict(batch=Sq * Skv, query=Skv))
     check(got, *attention(c.q, k, v, lens, bias), f"many rows d={d} {kind}")
+
+
+@pytest.mark.parametrize("dt", [F16, F32])
+@pytest.mark.parametrize("B,Hk,G,Sq,Skv,d", [(2, 3, 1, 700, 150, 40), (3, 2, 2, 333, 97, 64), (1, 5, 1, 520, 300, 128)])
+def test_one_bias_for_many_heads(dev, rng, dt, B, Hk, G, Sq, Skv, d):
+    """Many blocks of rows under few heads, which then go side by side."""
+    c = Case(dev, rng, B, Hk * G, Hk, Sq, Skv, d, dt)
+    bias = rng.standard_normal((B, 1, Sq, Skv)).astype(np.float32)
+    bias[:, :, 100:110, :60] = -np.inf
+    bias[:, :, 3] = -np.inf
+    bias[:, :, 200, 5:9] = -2e30
+    lens = [Skv - 7 * i for i in range(B)]
+    k, v = c.kv()
+    got = c.run(lens=lens, bias=bias, bias_strides=dict(batch=Sq * Skv, query=Skv))
+    check(got, *attention(c.q, k, v, lens, bias, dt=dt), f"one bias d={d}")
+    assert not got[:, :, 3].any()
