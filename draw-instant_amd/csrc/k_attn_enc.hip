@@ -29,7 +29,7 @@ extern "C" int32_t di_attn_encoder(di_ctx* ctx, const di_heads* q, const di_head
              fn, B, Hq, Hk, Sq, Skv, d);
   DI_REQUIRE(Hq % Hk == 0, DI_EINVAL, "%s: %u query heads over %u key heads", fn, Hq, Hk);
   DI_REQUIRE(d % 8 == 0 && d <= 256, DI_EUNSUPPORTED, "%s: head dim %u (a multiple of 8 up to 256)", fn, d);
-  DI_REQUIRE(std::isfinite(scale), DI_EINVAL, "%s: scale %g", fn, (double)scale);
+  DI_REQUIRE(std::isfinite(scale * kLog2E), DI_EINVAL, "%s: scale %g", fn, (double)scale);
   DI_REQUIRE(Skv < 1u << 31, DI_EUNSUPPORTED, "%s: %u keys", fn, Skv);
   HeadsPtr pq, pk, pv, po;
   int rc = check_heads(ctx, q, fn, "q", B, Sq, Hq, d, dt, &pq);

@@ -66,6 +66,7 @@ static void attention() {
   REFUSE(DI_EINVAL, "dtype", c.dt = 2);
   REFUSE(DI_EINVAL, "scale", c.scale = NAN);
   REFUSE(DI_EINVAL, "scale", c.scale = INFINITY);
+  REFUSE(DI_EINVAL, "scale", c.scale = 3e38f);
   REFUSE(DI_EHANDLE, "handle", c.q.buf = 0);
   REFUSE(DI_EHANDLE, "handle", c.v.buf = 12345);
   REFUSE(DI_EHANDLE, "handle", c.len = 12345);
